@@ -530,6 +530,43 @@ int igr_layer_tail_bwd_f32(int64_t n, int32_t d, const float *gn, int64_t ldgn, 
                            const float *r, const float *row_norm, const float *keep, float keep_scale,
                            float slope, float *dz, void *stream);
 
+/* ------------------------------------------------------- catalogue loss */
+
+/* Element types of the entry points below that take more than fp32. */
+#define IGR_DTYPE_F32 0
+#define IGR_DTYPE_BF16 1
+#define IGR_DTYPE_F16 2
+
+/* Softmax cross entropy of b batch rows against all v items, without the logits in memory:
+ *   s_bv = scale <x_b, items_v>,   loss_b = log sum_v exp(s_bv) - s_b,target(b)
+ * Rows whose target is ignore_index have loss 0 and take no part in any gradient, whatever
+ * they hold; a target that is neither ignore_index nor in [0, v) gives NaN.  x [b, d] and
+ * items [v, d] are of `dtype`, unit inner stride, 0 < d <= 256, any alignment; scale > 0.
+ *   x_pack, item_pack  igr_softmax_loss_pack_size bytes each, 16-byte aligned: the tables as
+ *                      matrix fragments, written here and read by the backward
+ *   loss, lse2 [b]     the rows' losses and log2 of the sums
+ *   total, count       (both or neither) the sum, with `mean` the mean, of the losses over the
+ *                      rows that are not ignored (0 if there are none), and their number
+ *   o                  [b, 32 / 64 / 128 / 256 - the next that holds d] rows of
+ *                      sum_v softmax_bv items_v for dx; NULL if dx will not be asked for
+ * The workspace holds igr_softmax_loss_workspace_size(b, v, d, 0, o != NULL) bytes.  fp32
+ * products run on the 16-bit matrix cores in three parts with fp32's accuracy; half types
+ * multiply as they are and round the softmax weights once.  Fixed summation order. */
+int64_t igr_softmax_loss_pack_size(int64_t rows, int32_t d, int32_t dtype);
+int64_t igr_softmax_loss_workspace_size(int64_t b, int64_t v, int32_t d, int32_t backward, int32_t with_o);
+int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *x, int64_t ldx,
+                         const void *items, int64_t ld_items, const int64_t *target, int64_t ignore_index,
+                         float scale, int32_t mean, void *x_pack, void *item_pack, float *loss, float *lse2,
+                         float *total, float *count, float *o, void *workspace, int64_t ws_bytes, void *stream);
+/* Its gradients: dx [b, d] and dw [v, d] of `dtype`, contiguous, either NULL.  grad: one
+ * device float (the total's gradient), or with per_row one per row; `mean` divides by *count.
+ * The workspace holds igr_softmax_loss_workspace_size(b, v, d, 1, 0) bytes. */
+int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *items, int64_t ld_items,
+                         const int64_t *target, int64_t ignore_index, float scale, int32_t mean, int32_t per_row,
+                         const float *grad, const void *x_pack, const void *item_pack, const float *lse2,
+                         const float *count, const float *o, void *dx, void *dw, void *workspace,
+                         int64_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

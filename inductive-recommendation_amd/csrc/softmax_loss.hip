@@ -1,0 +1,927 @@
+// softmax_loss.hip - softmax cross entropy over a whole item catalogue, and its gradients,
+// without ever holding the logits (gfx950 matrix cores).
+//
+//   s_bv   = scale <x_b, w_v>                       b < B batch rows, v < V items, width d <= 256
+//   loss_b = log sum_v exp(s_bv) - s_b,t(b)         0 for rows whose target is ignore_index
+//   dx_b   = c_b (o_b - w_t(b)),  o_b = sum_v p_bv w_v,  p_bv = exp(s_bv - lse_b)
+//   dw_v   = sum_b c_b (p_bv - [v = t(b)]) x_b,     c_b = scale d(total)/d(loss_b)
+//
+// o_b does not depend on the incoming gradient, so the forward pass computes it along with the
+// running maximum and sum (each tile of logits is used for both and dropped); the backward
+// recomputes the logits once, for dw.  That is 8 B V d flops in all, where the logits
+// kept would need 6 and B V floats.
+//
+// Layout.  Both tables are first packed into 16-bit matrix fragments (half_split.h), per block
+// of 32 rows: an S part (contraction over the width: lane l holds row l % 32, eight
+// consecutive columns) and a T part (contraction over the rows: lane l holds column l % 32
+// and eight rows, in exactly the order in which a 32x32 MFMA leaves its results in a lane).
+// So the weights p of one product are, in the registers they were made in, the operand of the next,
+// and a tile is copied to LDS and read back as it lies, 16 bytes a lane, without conflicts.
+//
+// Forward: a workgroup of four waves holds 32 NB batch rows a wave in registers and streams a range of
+// item blocks; few batch rows split the catalogue over many workgroups, whose (max, sum, o) are
+// joined in split order.  Backward: the same with the roles exchanged, item rows
+// in registers and batch blocks streamed; no atomics, the same bits on every run.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "half_split.h"
+
+namespace igr {
+namespace {
+
+constexpr int kRB = 32;       // rows of a packed block
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int64_t kWantGroups = 512;  // two workgroups on each of 256 CUs
+
+inline int pad_width(int32_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+__host__ __device__ inline int64_t blocks_of(int64_t rows) { return (rows + kRB - 1) / kRB; }
+// 16-bit values of one packed block: S part and T part of NS planes
+template <class P>
+__host__ __device__ constexpr int block_halves(int dp) { return 2 * P::NS * kRB * dp; }
+inline int64_t block_bytes(int32_t dtype, int dp) { return (dtype == kF32 ? 2 : 1) * 2ll * kRB * dp * 2; }
+inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
+
+// A packed table: its blocks, then one exponent per block.
+struct Packed {
+    const uint4 *blocks;
+    const int32_t *exps;
+};
+inline Packed packed_view(const void *p, int64_t rows, int32_t dtype, int dp) {
+    const char *c = static_cast<const char *>(p);
+    return Packed{reinterpret_cast<const uint4 *>(c),
+                  reinterpret_cast<const int32_t *>(c + blocks_of(rows) * block_bytes(dtype, dp))};
+}
+
+struct PackArgs {
+    int64_t rows, ld;
+    const void *src;
+    uint4 *blocks;
+    int32_t *exps;
+    const int64_t *target;  // rows whose target is `ignore` are packed as zeros; NULL: none
+    int64_t ignore;
+};
+
+// One block of 32 rows per workgroup; bound by its traffic (a table row is read once and written
+// twice, as S and T fragments).
+template <class P, int DP>
+__global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, int64_t n0, int32_t d, int32_t vec) {
+    __shared__ float tile[kRB][DP + 1];
+    __shared__ float wmax[kThreads / 64];
+    const int64_t blk = blockIdx.x < n0 ? blockIdx.x : blockIdx.x - n0;
+    const PackArgs a = blockIdx.x < n0 ? a0 : a1;
+    const typename P::elem *src = static_cast<const typename P::elem *>(a.src);
+    const int64_t r0 = blk * kRB;
+    const int t = threadIdx.x;
+    constexpr int VE = 16 / sizeof(typename P::elem);
+    float amax = 0.f;
+    auto put = [&](int r, int c, float v) {
+        tile[r][c] = v;
+        const float m = fabsf(v);
+        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);  // finite entries set the scale
+    };
+    if (vec) {  // rows of whole 16-byte groups
+        for (int i = t; i < kRB * DP / VE; i += kThreads) {
+            const int r = i / (DP / VE), c = (i % (DP / VE)) * VE;
+            const int64_t gr = r0 + r;
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (gr < a.rows && c < d && !(a.target && a.target[gr] == a.ignore))
+                raw = *reinterpret_cast<const uint4 *>(src + gr * a.ld + c);
+            typename P::elem e[VE];
+            __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+            for (int j = 0; j < VE; ++j) put(r, c + j, (float)e[j]);
+        }
+    } else {
+        for (int i = t; i < kRB * DP; i += kThreads) {
+            const int r = i / DP, c = i % DP;
+            const int64_t gr = r0 + r;
+            float v = 0.f;
+            if (gr < a.rows && c < d && !(a.target && a.target[gr] == a.ignore)) v = (float)src[gr * a.ld + c];
+            put(r, c, v);
+        }
+    }
+    int e = 0;
+    float s = 1.f;
+    if constexpr (P::kScaled) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+        if ((t & 63) == 0) wmax[t >> 6] = amax;
+    }
+    __syncthreads();
+    if constexpr (P::kScaled) {
+        e = block_exponent(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])));
+        s = pow2f(P::kOff - e);
+    }
+    if (t == 0) a.exps[blk] = e;
+    uint4 *out = a.blocks + blk * (block_halves<P>(DP) / 8);
+    constexpr int KS = DP / 16, DB = DP / 32;
+    const int lane = t & 63, col = lane & 31, h = lane >> 5;
+    for (int f = t >> 6; f < 2 * KS; f += kThreads / 64) {
+        float v[8];
+        if (f < KS) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = tile[col][f * 16 + h * 8 + i] * s;
+        } else {
+            const int g = f - KS, db = g >> 1, st = g & 1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = tile[16 * st + 8 * (i >> 2) + 4 * h + (i & 3)][db * 32 + col] * s;
+        }
+        Frags<P> fr;
+        split8(v, fr);
+#pragma unroll
+        for (int n = 0; n < P::NS; ++n) out[(f * P::NS + n) * 64 + lane] = __builtin_bit_cast(uint4, fr.p[n]);
+    }
+    static_assert(DB * 2 == KS, "T part has as many fragments as the S part");
+}
+
+template <class P>
+__device__ __forceinline__ void load_frags(const uint4 *base, int f, int lane, Frags<P> &fr) {
+#pragma unroll
+    for (int n = 0; n < P::NS; ++n)
+        fr.p[n] = __builtin_bit_cast(typename P::frag, base[(f * P::NS + n) * 64 + lane]);
+}
+
+struct FwdArgs {
+    int64_t B, V, nbt, splits, per;  // batch tiles, catalogue splits, item blocks per split
+    Packed x, w;
+    const int64_t *target;
+    float scale2;  // scale log2(e)
+    float *pm, *pz, *pt, *po;  // partials: [splits][B] max (log2), sum, target logit; [splits][B][DP]
+    int32_t *pc;               // [splits] exponent of po
+};
+
+// WITH_O = false: the loss alone (no product with the T part, which is then not copied either).
+template <class P, int DP, int NB, bool WITH_O>
+__global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdArgs a) {
+    constexpr int KS = DP / 16, DB = DP / 32;
+    constexpr int TILE = block_halves<P>(DP) / 8 / (WITH_O ? 1 : 2);  // uint4 of a streamed block
+    constexpr int BLK = block_halves<P>(DP) / 8;
+    constexpr int NST = (TILE + kThreads - 1) / kThreads;
+    __shared__ uint4 lds[2][TILE];
+    __shared__ int32_t cmax_s;
+    // workgroups of one split sit on one XCD (blockIdx % 8), next to each other in time: the
+    // split's item blocks come from that XCD's L2 for all batch tiles but the first
+    const int64_t id = blockIdx.x, xcd = id & 7, j = id >> 3;
+    const int64_t split = (j / a.nbt) * 8 + xcd, bt = j % a.nbt;
+    if (split >= a.splits) return;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
+    const int64_t nblk = blocks_of(a.V);
+    const int64_t k0 = split * a.per, k1 = k0 + a.per < nblk ? k0 + a.per : nblk;
+    const int64_t nxb = blocks_of(a.B);
+
+    // exponent that the weights of the split's blocks are made for: the largest of the split's blocks
+    int C = 0;
+    if constexpr (P::kScaled) {
+        if (t == 0) cmax_s = -127;
+        __syncthreads();
+        int c = -127;
+        for (int64_t k = k0 + t; k < k1; k += kThreads) c = max(c, a.w.exps[k]);
+        atomicMax(&cmax_s, c);  // in LDS; a maximum does not depend on the order
+        __syncthreads();
+        C = __builtin_amdgcn_readfirstlane(cmax_s);
+    }
+
+    // this wave's batch blocks
+    Frags<P> xf[NB][KS];
+    float c_x[NB], m[NB], z[NB], tl[NB];
+    int tgt[NB];
+    bool live[NB];
+    f32x16_t o[NB][WITH_O ? DB : 1];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int64_t xb = (bt * 4 + wave) * NB + n;
+        live[n] = xb < nxb;
+        const int64_t xs = live[n] ? xb : 0;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) load_frags<P>(a.x.blocks + xs * BLK, k, lane, xf[n][k]);
+        c_x[n] = a.scale2 * (P::kScaled ? pow2f(a.x.exps[xs] - P::kOff) : 1.f);
+        m[n] = -INFINITY;
+        z[n] = 0.f;
+        tl[n] = 0.f;
+        const int64_t b = xs * kRB + col;
+        const int64_t tt = live[n] && b < a.B ? a.target[b] : -1;
+        tgt[n] = tt >= 0 && tt < a.V ? (int)tt : -1;
+#pragma unroll
+        for (int q = 0; q < (WITH_O ? DB : 1); ++q)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[n][q][i] = 0.f;
+    }
+
+    uint4 st[NST];
+    auto fetch = [&](int64_t k) {
+        const uint4 *src = a.w.blocks + k * BLK;
+#pragma unroll
+        for (int i = 0; i < NST; ++i)
+            if (TILE % kThreads == 0 || i * kThreads + t < TILE) st[i] = src[i * kThreads + t];
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NST; ++i)
+            if (TILE % kThreads == 0 || i * kThreads + t < TILE) lds[buf][i * kThreads + t] = st[i];
+    };
+    fetch(k0);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (int64_t k = k0; k < k1; ++k, buf ^= 1) {
+        if (k + 1 < k1) fetch(k + 1);
+        const uint4 *w = lds[buf];
+        const int ew = P::kScaled ? __builtin_amdgcn_readfirstlane(a.w.exps[k]) : 0;
+        const float c_w = P::kScaled ? pow2f(ew - P::kOff) : 1.f;
+        f32x16_t acc[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            Frags<P> wf;
+            load_frags<P>(w, s, lane, wf);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) acc[n] = mfma_split<P>(wf, xf[n][s], acc[n]);
+        }
+        const int v0 = (int)(k * kRB);
+        const int nv = a.V - k * kRB < kRB ? (int)(a.V - k * kRB) : kRB;  // items of this block
+        Frags<P> pf[NB][2];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            // lane: batch row `col` of block n; register i: item 8 (i/4) + 4 h + i%4
+            const float c = c_x[n] * c_w;
+            if (__any((unsigned)(tgt[n] - v0) < 32u)) {  // some row's target is here: keep its logit
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (tgt[n] - v0 == 8 * (i >> 2) + 4 * h + (i & 3)) tl[n] = acc[n][i] * c;
+            }
+            if (nv < kRB) {  // the catalogue's last block: its padding takes no part
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (8 * (i >> 2) + 4 * h + (i & 3) >= nv) acc[n][i] = -INFINITY;
+            }
+            float mx = acc[n][0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[n][i]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+            if (__any(mx > m[n])) {  // rare after the first blocks
+                const float mn = fmaxf(m[n], mx);
+                const float f = __builtin_amdgcn_exp2f(m[n] - mn);
+                m[n] = mn;
+                z[n] *= f;
+                if constexpr (WITH_O) {
+#pragma unroll
+                    for (int q = 0; q < DB; ++q)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[n][q][i] *= f;
+                }
+            }
+            // weights p 2^sh: up to 2^14 in the halves' range, less where the block's rows are
+            // smaller than the split's largest.  -60 keeps the sum exact; a block that far
+            // below adds nothing to o either way.
+            // (without o the same powers, for the same sums bit for bit)
+            const int sh = 14 + (P::kScaled ? max(ew - C, -60) : 0);
+            const float off = m[n] - (float)sh;
+            float p[16];
+            if (nv < kRB) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < nv ? __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off)) : 0.f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
+            }
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                s0 += p[i];
+                s1 += p[i + 1];
+            }
+            z[n] = fmaf(s0 + s1, pow2f(-sh), z[n]);
+            if constexpr (WITH_O) {
+                float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
+                float (&ph)[8] = reinterpret_cast<float (&)[8]>(p[8]);
+                split8(pl, pf[n][0]);
+                split8(ph, pf[n][1]);
+            }
+        }
+        if constexpr (WITH_O) {
+#pragma unroll
+            for (int q = 0; q < DB; ++q)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    Frags<P> wf;
+                    load_frags<P>(w, KS + 2 * q + s, lane, wf);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) o[n][q] = mfma_split<P>(wf, pf[n][s], o[n][q]);
+                }
+        }
+        if (k + 1 < k1) stage(buf ^ 1);
+        __syncthreads();
+    }
+    if (WITH_O && bt == 0 && t == 0) a.pc[split] = C;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int64_t b = ((bt * 4 + wave) * NB + n) * kRB + col;
+        // the two halves of a row: same maximum, sums of different items, one target logit
+        const float zz = z[n] + __shfl_xor(z[n], 32, 64);
+        const float ot = __shfl_xor(tl[n], 32, 64);
+        const bool mine = (tgt[n] >> 2 & 1) == h;  // items 8q + 4h + 0..3 are this half's
+        if (!live[n] || b >= a.B) continue;
+        if (h == 0) {
+            a.pm[split * a.B + b] = m[n];
+            a.pz[split * a.B + b] = zz;
+            a.pt[split * a.B + b] = mine ? tl[n] : ot;
+        }
+        if constexpr (WITH_O) {
+            float *dst = a.po + (split * a.B + b) * DP;
+#pragma unroll
+            for (int q = 0; q < DB; ++q)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<float4 *>(dst + q * 32 + g * 8 + h * 4) =
+                        make_float4(o[n][q][4 * g], o[n][q][4 * g + 1], o[n][q][4 * g + 2], o[n][q][4 * g + 3]);
+        }
+    }
+}
+
+struct JoinArgs {
+    int64_t B, V, splits, per;
+    int32_t d, ooff;  // ooff: po carries 2^(ooff - C)
+    const float *pm, *pz, *pt, *po;
+    const int32_t *pc;
+    const int64_t *target;
+    int64_t ignore;
+    float *loss, *lse2, *o;  // o: [B, DP] or NULL
+};
+
+// One batch row per workgroup: the splits' (max, sum, o) joined in split order, a quarter of them
+// per wave.  Reads the partials once.
+template <int DP>
+__global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
+    __shared__ float part[4][DP];
+    __shared__ float wm[4], wz[4];
+    const int64_t b = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int64_t tg = a.target[b];
+    if (tg == a.ignore) {
+        if (t == 0) {
+            a.loss[b] = 0.f;
+            a.lse2[b] = 0.f;
+        }
+        if (a.o)
+            for (int c = t; c < DP; c += kThreads) a.o[b * DP + c] = 0.f;
+        return;
+    }
+    float m = -INFINITY;
+    for (int64_t s = t; s < a.splits; s += kThreads) m = fmaxf(m, a.pm[s * a.B + b]);
+#pragma unroll
+    for (int q = 32; q; q >>= 1) m = fmaxf(m, __shfl_xor(m, q, 64));
+    if (lane == 0) wm[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    float z = 0.f;
+    for (int64_t s = t; s < a.splits; s += kThreads)
+        z += a.pz[s * a.B + b] * __builtin_amdgcn_exp2f(a.pm[s * a.B + b] - m);
+#pragma unroll
+    for (int q = 32; q; q >>= 1) z += __shfl_xor(z, q, 64);
+    if (lane == 0) wz[wave] = z;
+    __syncthreads();
+    z = (wz[0] + wz[1]) + (wz[2] + wz[3]);
+    if (t == 0) {
+        float loss = NAN;  // a target that names no item
+        if (tg >= 0 && tg < a.V) {
+            const float st = a.pt[(tg / kRB / a.per) * a.B + b];
+            loss = kLn2 * (m - st) + logf(z);  // both terms >= 0 up to rounding: no cancellation
+            loss = loss < 0.f ? 0.f : loss;
+        }
+        a.loss[b] = loss;
+        a.lse2[b] = m + log2f(z);
+    }
+    if (!a.o) return;
+    const int64_t q0 = a.splits * wave / 4, q1 = a.splits * (wave + 1) / 4;
+    constexpr int NC = (DP + 63) / 64;
+    float acc[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = 0.f;
+#pragma unroll 4
+    for (int64_t s = q0; s < q1; ++s) {
+        const float f = __builtin_amdgcn_exp2f(a.pm[s * a.B + b] - m) * ldexpf(1.f, a.pc[s] - a.ooff);
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (c * 64 + lane < DP) acc[c] = fmaf(a.po[(s * a.B + b) * DP + c * 64 + lane], f, acc[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+        if (c * 64 + lane < DP) part[wave][c * 64 + lane] = acc[c];
+    __syncthreads();
+    for (int c = t; c < DP; c += kThreads)
+        a.o[b * DP + c] = ((part[0][c] + part[1][c]) + (part[2][c] + part[3][c])) / z;
+}
+
+// The loss's sum or mean over the rows that are not ignored, and their number.
+__global__ __launch_bounds__(kThreads) void softmax_reduce(int64_t B, const float *loss, const int64_t *target,
+                                                           int64_t ignore, int32_t mean, float *total,
+                                                           float *count) {
+    __shared__ double ss[kThreads];
+    __shared__ int64_t sn[kThreads];
+    const int t = threadIdx.x;
+    double s = 0.;
+    int64_t n = 0;
+    for (int64_t b = t; b < B; b += kThreads) {
+        s += loss[b];
+        n += target[b] != ignore;
+    }
+    ss[t] = s;
+    sn[t] = n;
+    __syncthreads();
+    for (int w = kThreads / 2; w; w >>= 1) {
+        if (t < w) {
+            ss[t] += ss[t + w];
+            sn[t] += sn[t + w];
+        }
+        __syncthreads();
+    }
+    if (t == 0) {
+        *total = (float)(mean ? ss[0] / (double)(sn[0] > 0 ? sn[0] : 1) : ss[0]);
+        *count = (float)sn[0];
+    }
+}
+
+// What the streamed batch blocks of the backward carry besides their fragments, per row: the
+// exponent offset that makes exp2(acc c - off) = |c_b| p 2^(14 + e - C), the same power of c_b for
+// the target's own term, the target.
+struct RowInfo {
+    float *off, *hot;
+    int32_t *tgt;
+    int32_t *neg;   // per block: some c_b < 0
+    int32_t *cmax;  // C: the largest e + floor(log2 |c_b|)
+};
+
+struct CoefArgs {
+    int64_t B, V;
+    int32_t d, per_row, mean;
+    const float *grad, *count, *lse2, *o;
+    const int64_t *target;
+    int64_t ignore;
+    float scale;
+    Packed x;
+    RowInfo info;
+    int64_t n_info;    // workgroups that fill the row info (0: dw is not wanted)
+    const void *items; // for dx
+    int64_t ld_items;
+    void *dx;
+};
+
+__device__ __forceinline__ float row_coef(const CoefArgs &a, int64_t b, int64_t tg) {
+    if (tg == a.ignore) return 0.f;
+    if (tg < 0 || tg >= a.V) return NAN;
+    const float g = (a.per_row ? a.grad[b] : a.grad[0]) * a.scale;
+    return a.mean ? g / fmaxf(*a.count, 1.f) : g;
+}
+
+// Workgroups below n_info: the row info of 256 rows.  The others: dx of four rows, one a wave.
+template <class T, int DP, bool SCALED>
+__global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    if ((int64_t)blockIdx.x >= a.n_info) {
+        const int64_t b = ((int64_t)blockIdx.x - a.n_info) * 4 + wave;
+        if (b >= a.B) return;
+        const int64_t tg = a.target[b];
+        const float c = row_coef(a, b, tg);
+        const bool ok = tg != a.ignore;
+        const T *w = static_cast<const T *>(a.items) + (tg >= 0 && tg < a.V ? tg : 0) * a.ld_items;
+        T *dx = static_cast<T *>(a.dx) + b * a.d;
+        for (int q = lane; q < a.d; q += 64) dx[q] = ok ? (T)(c * (a.o[b * DP + q] - (float)w[q])) : (T)0.f;
+        return;
+    }
+    __shared__ int32_t cm;
+    if (t == 0) cm = -250;
+    __syncthreads();
+    int c_all = -250;
+    for (int64_t b = t; b < a.B; b += kThreads) {
+        const float c = fabsf(row_coef(a, b, a.target[b]));
+        if (c > 0.f) c_all = max(c_all, block_exponent(c) + (SCALED ? a.x.exps[b / kRB] : 0));
+    }
+    atomicMax(&cm, c_all);  // in LDS; a maximum does not depend on the order
+    __syncthreads();
+    const int C = cm;
+    const int64_t b = (int64_t)blockIdx.x * kThreads + t;
+    if (b >= blocks_of(a.B) * kRB) return;
+    float off = INFINITY, hot = 0.f;
+    int tgt = -1;
+    if (b < a.B) {
+        const int64_t tg = a.target[b];
+        const float c = row_coef(a, b, tg);
+        const int e = SCALED ? a.x.exps[b / kRB] : 0;
+        if (c != 0.f) {
+            off = a.lse2[b] - log2f(fabsf(c)) - (float)(14 + e - C);
+            hot = ldexpf(c, 14 + e - C);
+            tgt = tg >= 0 && tg < a.V ? (int)tg : -1;
+        }
+    }
+    a.info.off[b] = off;
+    a.info.hot[b] = hot;
+    a.info.tgt[b] = tgt;
+    const uint64_t neg = __ballot(hot < 0.f);
+    if ((lane & 31) == 0) a.info.neg[b / kRB] = (uint32_t)(neg >> lane) != 0;
+    if (b == 0) *a.info.cmax = C;
+}
+
+struct BwdArgs {
+    int64_t B, V, splits, per;  // batch splits, batch blocks per split
+    int32_t d, vec;
+    Packed x, w;
+    RowInfo info;
+    float scale2;
+    void *dw;
+    float *part;  // [splits][V][DP] when splits > 1
+};
+
+template <class T>
+__device__ __forceinline__ void store4(T *dst, int c, int d, bool vec, float a, float b, float e, float f) {
+    if (vec) {  // d and the leading dimension are multiples of 4
+        if (c < d) {
+            T v[4] = {(T)a, (T)b, (T)e, (T)f};
+            __builtin_memcpy(__builtin_assume_aligned(dst + c, 4 * sizeof(T)), v, sizeof v);
+        }
+        return;
+    }
+    if (c < d) dst[c] = (T)a;
+    if (c + 1 < d) dst[c + 1] = (T)b;
+    if (c + 2 < d) dst[c + 2] = (T)e;
+    if (c + 3 < d) dst[c + 3] = (T)f;
+}
+
+// dw of 32 NB items a wave: logits recomputed tile by tile, weights times batch rows accumulated.
+template <class P, int DP, int NB>
+__global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdArgs a) {
+    constexpr int KS = DP / 16, DB = DP / 32;
+    constexpr int BLK = block_halves<P>(DP) / 8;
+    constexpr int NST = (BLK + kThreads - 1) / kThreads;
+    __shared__ uint4 lds[2][BLK];
+    __shared__ float info[2][3][kRB];  // off, hot, target of the streamed block
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
+    const int64_t nvb = blocks_of(a.V), nxb = blocks_of(a.B);
+    const int64_t split = blockIdx.y;
+    const int64_t k0 = split * a.per, k1 = k0 + a.per < nxb ? k0 + a.per : nxb;
+
+    Frags<P> wf[NB][KS];
+    float c_w[NB];
+    int v0[NB];
+    bool live[NB];
+    f32x16_t o[NB][DB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int64_t vb = ((int64_t)blockIdx.x * 4 + wave) * NB + n;
+        live[n] = vb < nvb;
+        const int64_t vs = live[n] ? vb : 0;
+        v0[n] = (int)(vs * kRB);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) load_frags<P>(a.w.blocks + vs * BLK, k, lane, wf[n][k]);
+        c_w[n] = a.scale2 * (P::kScaled ? pow2f(a.w.exps[vs] - P::kOff) : 1.f);
+#pragma unroll
+        for (int q = 0; q < DB; ++q)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[n][q][i] = 0.f;
+    }
+
+    uint4 st[NST];
+    float si = 0.f;
+    auto fetch = [&](int64_t k) {
+        const uint4 *src = a.x.blocks + k * BLK;
+#pragma unroll
+        for (int i = 0; i < NST; ++i)
+            if (BLK % kThreads == 0 || i * kThreads + t < BLK) st[i] = src[i * kThreads + t];
+        if (t < kRB) si = a.info.off[k * kRB + t];
+        else if (t < 2 * kRB) si = a.info.hot[k * kRB + t - kRB];
+        else if (t < 3 * kRB) si = __builtin_bit_cast(float, a.info.tgt[k * kRB + t - 2 * kRB]);
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NST; ++i)
+            if (BLK % kThreads == 0 || i * kThreads + t < BLK) lds[buf][i * kThreads + t] = st[i];
+        if (t < 3 * kRB) info[buf][t / kRB][t % kRB] = si;
+    };
+    fetch(k0);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (int64_t k = k0; k < k1; ++k, buf ^= 1) {
+        if (k + 1 < k1) fetch(k + 1);
+        const uint4 *x = lds[buf];
+        const float c_x = P::kScaled ? pow2f(__builtin_amdgcn_readfirstlane(a.x.exps[k]) - P::kOff) : 1.f;
+        const bool neg = __builtin_amdgcn_readfirstlane(a.info.neg[k]) != 0;
+        f32x16_t acc[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            Frags<P> xf;
+            load_frags<P>(x, s, lane, xf);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) acc[n] = mfma_split<P>(xf, wf[n][s], acc[n]);
+        }
+        // lane: item v0 + col; register i: batch row 8 (i/4) + 4 h + i%4 of the block
+        float off[16];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 f = *reinterpret_cast<const float4 *>(&info[buf][0][8 * g + 4 * h]);
+            off[4 * g] = f.x;
+            off[4 * g + 1] = f.y;
+            off[4 * g + 2] = f.z;
+            off[4 * g + 3] = f.w;
+        }
+        const int tcol = __builtin_bit_cast(int, info[buf][2][col]);
+        Frags<P> pf[NB][2];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float c = c_w[n] * c_x;
+            float p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off[i]));
+            if (neg) {  // a negative c_b: only where the caller's gradients are
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = copysignf(p[i], info[buf][1][8 * (i >> 2) + 4 * h + (i & 3)]);
+            }
+            if (__any((unsigned)(tcol - v0[n]) < 32u)) {  // some row's target is one of these items
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (__builtin_bit_cast(int, info[buf][2][r]) == v0[n] + col) p[i] -= info[buf][1][r];
+                }
+            }
+            float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
+            float (&ph)[8] = reinterpret_cast<float (&)[8]>(p[8]);
+            split8(pl, pf[n][0]);
+            split8(ph, pf[n][1]);
+        }
+#pragma unroll
+        for (int q = 0; q < DB; ++q)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                Frags<P> xf;
+                load_frags<P>(x, KS + 2 * q + s, lane, xf);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[n][q] = mfma_split<P>(xf, pf[n][s], o[n][q]);
+            }
+        if (k + 1 < k1) stage(buf ^ 1);
+        __syncthreads();
+    }
+    const float f = a.splits > 1 ? 1.f : ldexpf(1.f, *a.info.cmax - 14 - P::kOff);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int64_t v = (int64_t)v0[n] + col;
+        if (!live[n] || v >= a.V) continue;
+#pragma unroll
+        for (int q = 0; q < DB; ++q)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = q * 32 + g * 8 + h * 4;
+                const float w0 = o[n][q][4 * g] * f, w1 = o[n][q][4 * g + 1] * f, w2 = o[n][q][4 * g + 2] * f,
+                            w3 = o[n][q][4 * g + 3] * f;
+                if (a.splits > 1)
+                    *reinterpret_cast<float4 *>(a.part + (split * a.V + v) * DP + c) = make_float4(w0, w1, w2, w3);
+                else
+                    store4(static_cast<typename P::elem *>(a.dw) + v * a.d, c, a.d, a.vec, w0, w1, w2, w3);
+            }
+    }
+}
+
+// dw from the batch splits' partials, in split order.
+template <class T, int DP>
+__global__ __launch_bounds__(kThreads) void softmax_bwd_join(int64_t V, int32_t d, int64_t splits, int32_t off,
+                                                             const int32_t *cmax, const float *part, int32_t vec,
+                                                             T *dw) {
+    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    const int64_t v = i / (DP / 4);
+    const int c = (int)(i % (DP / 4)) * 4;
+    if (v >= V || c >= d) return;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t k = 0; k < splits; ++k)
+        s = f4_add(s, *reinterpret_cast<const float4 *>(part + (k * V + v) * DP + c));
+    s = f4_scale(ldexpf(1.f, *cmax - off), s);
+    store4(dw + v * d, c, d, vec, s.x, s.y, s.z, s.w);
+}
+
+// ------------------------------------------------------------------ host side
+
+struct FwdPlan {
+    int nb;
+    int64_t nbt, splits, per;
+};
+// Two blocks of batch rows a wave where they fit the registers of two workgroups on a CU and there
+// are that many rows: a streamed block then serves twice the rows.
+inline FwdPlan fwd_plan(int64_t B, int64_t V, int dp) {
+    FwdPlan p;
+    p.nb = dp <= 64 && B > 4 * kRB ? 2 : 1;
+    p.nbt = (blocks_of(B) + 4 * p.nb - 1) / (4 * p.nb);
+    const int64_t nblk = blocks_of(V);
+    p.per = std::max<int64_t>(1, (nblk * p.nbt + kWantGroups - 1) / kWantGroups);
+    p.splits = (nblk + p.per - 1) / p.per;
+    return p;
+}
+inline FwdPlan bwd_plan(int64_t B, int64_t V, int dp) {
+    FwdPlan p;
+    p.nb = dp <= 64 && blocks_of(V) >= 8 * kWantGroups ? 2 : 1;
+    p.nbt = (blocks_of(V) + 4 * p.nb - 1) / (4 * p.nb);
+    const int64_t nblk = blocks_of(B);
+    p.per = std::max<int64_t>(1, (nblk * p.nbt + kWantGroups - 1) / kWantGroups);
+    p.splits = (nblk + p.per - 1) / p.per;
+    return p;
+}
+
+inline int check_shape(const char *fn, int32_t dtype, int64_t b, int64_t v, int32_t d) {
+    if (dtype < kF32 || dtype > kF16) return arg_error(fn, "unknown dtype");
+    if (b < 0 || v <= 0 || d <= 0) return arg_error(fn, "sizes must be positive");
+    if (d > 256) {
+        set_error(std::string(fn) + ": width above 256");
+        return IGR_ERR_UNSUPPORTED;
+    }
+    if (v > INT32_MAX - 64 || b > INT32_MAX - 64) return arg_error(fn, "more than 2^31 - 65 rows");
+    return IGR_OK;
+}
+
+struct Carve {  // a workspace cut into 256-byte aligned pieces
+    char *p;
+    int64_t used = 0;
+    template <class T>
+    T *take(int64_t n) {
+        T *r = reinterpret_cast<T *>(p + used);
+        used += align256(n * (int64_t)sizeof(T));
+        return r;
+    }
+};
+
+template <class F>
+int by_type_width(int32_t dtype, int dp, F &&f) {
+    auto w = [&](auto pol) {
+        switch (dp) {
+            case 32: return f(pol, std::integral_constant<int, 32>());
+            case 64: return f(pol, std::integral_constant<int, 64>());
+            case 128: return f(pol, std::integral_constant<int, 128>());
+            default: return f(pol, std::integral_constant<int, 256>());
+        }
+    };
+    return dtype == kF32 ? w(SplitF32()) : dtype == kBF16 ? w(PlainBF16()) : w(PlainF16());
+}
+
+FwdArgs fwd_args(Carve &c, int64_t b, int64_t v, int dp, bool with_o) {
+    const FwdPlan p = fwd_plan(b, v, dp);
+    FwdArgs a{};
+    a.B = b, a.V = v, a.nbt = p.nbt, a.splits = p.splits, a.per = p.per;
+    a.pm = c.take<float>(p.splits * b);
+    a.pz = c.take<float>(p.splits * b);
+    a.pt = c.take<float>(p.splits * b);
+    a.pc = c.take<int32_t>(p.splits);
+    a.po = with_o ? c.take<float>(p.splits * b * dp) : nullptr;
+    return a;
+}
+
+BwdArgs bwd_args(Carve &c, int64_t b, int64_t v, int dp) {
+    const FwdPlan p = bwd_plan(b, v, dp);
+    BwdArgs a{};
+    a.B = b, a.V = v, a.splits = p.splits, a.per = p.per;
+    const int64_t rows = blocks_of(b) * kRB;
+    a.info.off = c.take<float>(rows);
+    a.info.hot = c.take<float>(rows);
+    a.info.tgt = c.take<int32_t>(rows);
+    a.info.neg = c.take<int32_t>(rows / kRB);
+    a.info.cmax = c.take<int32_t>(1);
+    a.part = p.splits > 1 ? c.take<float>(p.splits * v * dp) : nullptr;
+    return a;
+}
+
+}  // namespace
+}  // namespace igr
+
+using namespace igr;
+
+extern "C" int64_t igr_softmax_loss_pack_size(int64_t rows, int32_t d, int32_t dtype) {
+    if (rows <= 0 || d <= 0 || d > 256 || dtype < kF32 || dtype > kF16) return 0;
+    return align256(blocks_of(rows) * (block_bytes(dtype, pad_width(d)) + (int64_t)sizeof(int32_t)));
+}
+
+extern "C" int64_t igr_softmax_loss_workspace_size(int64_t b, int64_t v, int32_t d, int32_t backward, int32_t with_o) {
+    if (b <= 0 || v <= 0 || d <= 0 || d > 256) return 0;
+    Carve c{nullptr};
+    if (backward) bwd_args(c, b, v, pad_width(d));
+    else fwd_args(c, b, v, pad_width(d), with_o != 0);
+    return c.used;
+}
+
+extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *x, int64_t ldx,
+                                    const void *items, int64_t ld_items, const int64_t *target, int64_t ignore_index,
+                                    float scale, int32_t mean, void *x_pack, void *item_pack, float *loss, float *lse2,
+                                    float *total, float *count, float *o, void *workspace, int64_t ws_bytes, void *stream) {
+    return guarded("igr_softmax_loss_fwd", [&]() -> int {
+        const char *fn = "igr_softmax_loss_fwd";
+        if (int rc = check_shape(fn, dtype, b, v, d)) return rc;
+        if (ldx < d || ld_items < d) return arg_error(fn, "leading dimension too small");
+        if (!(scale > 0.f) || !std::isfinite(scale)) return arg_error(fn, "scale must be positive and finite");
+        if (b > 0 && (!items || !x_pack || !item_pack || !loss || !lse2 || !x || !target)) return arg_error(fn, "null pointer");
+        if (!total != !count) return arg_error(fn, "total and count go together");
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        if (b > 0) {
+            const int dp = pad_width(d);
+            Carve c{static_cast<char *>(workspace)};
+            FwdArgs a = fwd_args(c, b, v, dp, o != nullptr);
+            if (!workspace || ws_bytes < c.used || !aligned16(workspace) || !aligned16(x_pack) || !aligned16(item_pack))
+                return arg_error(fn, "workspace or pack too small or not 16-byte aligned");
+            a.x = packed_view(x_pack, b, dtype, dp);
+            a.w = packed_view(item_pack, v, dtype, dp);
+            a.target = target;
+            a.scale2 = scale * kLog2e;
+            const int64_t nx = blocks_of(b), nw = blocks_of(v), eb = dtype_bytes(dtype);
+            const bool vec = d * eb % 16 == 0 && ldx * eb % 16 == 0 && ld_items * eb % 16 == 0 && aligned16(x) &&
+                             aligned16(items);
+            PackArgs px{b, ldx, x, const_cast<uint4 *>(a.x.blocks), const_cast<int32_t *>(a.x.exps), target,
+                        ignore_index};
+            PackArgs pw{v, ld_items, items, const_cast<uint4 *>(a.w.blocks), const_cast<int32_t *>(a.w.exps), nullptr, 0};
+            const FwdPlan plan = fwd_plan(b, v, dp);
+            const int64_t grid = (a.splits + 7) / 8 * 8 * a.nbt;
+            if (grid > INT32_MAX || nx + nw > INT32_MAX) return arg_error(fn, "too many workgroups");
+            const int rc = by_type_width(dtype, dp, [&](auto pol, auto width) -> int {
+                using P = decltype(pol);
+                constexpr int DP = decltype(width)::value;
+                hipLaunchKernelGGL((pack_rows<P, DP>), dim3((unsigned)(nx + nw)), dim3(kThreads), 0, st, px, pw, nx, d,
+                                   (int32_t)vec);
+                const dim3 g((unsigned)grid);
+                if constexpr (DP <= 64) {
+                    if (plan.nb == 2) {
+                        if (o) hipLaunchKernelGGL((softmax_fwd<P, DP, 2, true>), g, dim3(kThreads), 0, st, a);
+                        else hipLaunchKernelGGL((softmax_fwd<P, DP, 2, false>), g, dim3(kThreads), 0, st, a);
+                    }
+                }
+                if (plan.nb == 1) {
+                    if (o) hipLaunchKernelGGL((softmax_fwd<P, DP, 1, true>), g, dim3(kThreads), 0, st, a);
+                    else hipLaunchKernelGGL((softmax_fwd<P, DP, 1, false>), g, dim3(kThreads), 0, st, a);
+                }
+                JoinArgs j{b, v, a.splits, a.per, d, 14 + P::kOff, a.pm, a.pz, a.pt, a.po, a.pc, target, ignore_index,
+                           loss, lse2, o};
+                hipLaunchKernelGGL((softmax_join<DP>), dim3((unsigned)b), dim3(kThreads), 0, st, j);
+                return IGR_OK;
+            });
+            if (rc) return rc;
+        }
+        if (total)
+            hipLaunchKernelGGL(softmax_reduce, dim3(1), dim3(kThreads), 0, st, b, loss, target, ignore_index, mean, total,
+                               count);
+        return launch_status(fn);
+    });
+}
+
+extern "C" int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *items,
+                                    int64_t ld_items, const int64_t *target, int64_t ignore_index, float scale,
+                                    int32_t mean, int32_t per_row, const float *grad, const void *x_pack,
+                                    const void *item_pack, const float *lse2, const float *count, const float *o, void *dx,
+                                    void *dw, void *workspace, int64_t ws_bytes, void *stream) {
+    return guarded("igr_softmax_loss_bwd", [&]() -> int {
+        const char *fn = "igr_softmax_loss_bwd";
+        if (int rc = check_shape(fn, dtype, b, v, d)) return rc;
+        if (ld_items < d) return arg_error(fn, "leading dimension too small");
+        if (!(scale > 0.f) || !std::isfinite(scale)) return arg_error(fn, "scale must be positive and finite");
+        if (b == 0 || (!dx && !dw)) return IGR_OK;
+        if (!target || !grad || !x_pack || !item_pack || !lse2 || (mean && !count) || (dx && (!o || !items)))
+            return arg_error(fn, "null pointer");
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        const int dp = pad_width(d);
+        Carve c{static_cast<char *>(workspace)};
+        BwdArgs a = bwd_args(c, b, v, dp);
+        if (!workspace || ws_bytes < c.used || !aligned16(workspace) || !aligned16(x_pack) || !aligned16(item_pack))
+            return arg_error(fn, "workspace or pack too small or not 16-byte aligned");
+        a.x = packed_view(x_pack, b, dtype, dp);
+        a.w = packed_view(item_pack, v, dtype, dp);
+        a.d = d;
+        a.vec = d % 4 == 0 && aligned16(dw);
+        a.scale2 = scale * kLog2e;
+        a.dw = dw;
+        const FwdPlan plan = bwd_plan(b, v, dp);
+        CoefArgs ca{b, v, d, per_row, mean, grad, count, lse2, o, target, ignore_index, scale, a.x, a.info,
+                    dw ? (blocks_of(b) * kRB + kThreads - 1) / kThreads : 0, items, ld_items, dx};
+        const int64_t cg = ca.n_info + (dx ? (b + 3) / 4 : 0);
+        if (plan.splits > 65535 || plan.nbt > INT32_MAX) return arg_error(fn, "too many workgroups");
+        const int rc = by_type_width(dtype, dp, [&](auto pol, auto width) -> int {
+            using P = decltype(pol);
+            using T = typename P::elem;
+            constexpr int DP = decltype(width)::value;
+            hipLaunchKernelGGL((softmax_coef<T, DP, P::kScaled>), dim3((unsigned)cg), dim3(kThreads), 0, st, ca);
+            if (!dw) return IGR_OK;
+            const dim3 g((unsigned)plan.nbt, (unsigned)plan.splits);
+            if constexpr (DP <= 64) {
+                if (plan.nb == 2) hipLaunchKernelGGL((softmax_bwd<P, DP, 2>), g, dim3(kThreads), 0, st, a);
+            }
+            if (plan.nb == 1) hipLaunchKernelGGL((softmax_bwd<P, DP, 1>), g, dim3(kThreads), 0, st, a);
+            if (plan.splits > 1)
+                hipLaunchKernelGGL((softmax_bwd_join<T, DP>), dim3((unsigned)((v * (DP / 4) + kThreads - 1) / kThreads)),
+                                   dim3(kThreads), 0, st, v, d, plan.splits, 14 + P::kOff, a.info.cmax, a.part,
+                                   (int32_t)a.vec, static_cast<T *>(dw));
+            return IGR_OK;
+        });
+        if (rc) return rc;
+        return launch_status(fn);
+    });
+}

@@ -126,6 +126,12 @@ SIGNATURES = {
     'igr_linear_wgrad_f32': (ctypes.c_int, [c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64,
                                             c_vp]),
     'igr_means_f32': (ctypes.c_int, [c_i64, c_vp, c_vp, c_vp, c_vp]),
+    'igr_softmax_loss_pack_size': (c_i64, [c_i64, c_i32, c_i32]),
+    'igr_softmax_loss_workspace_size': (c_i64, [c_i64, c_i64, c_i32, c_i32, c_i32]),
+    'igr_softmax_loss_fwd': (ctypes.c_int, [c_i32, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_f32,
+                                            c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    'igr_softmax_loss_bwd': (ctypes.c_int, [c_i32, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_f32, c_i32, c_i32,
+                                            c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     'igr_loss_combine_f32': (ctypes.c_int, [c_vp, c_vp, c_vp, c_f32, c_f32, c_f32, c_vp, c_vp, c_vp]),
 }
 

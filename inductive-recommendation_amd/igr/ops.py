@@ -1198,6 +1198,114 @@ def bpr_loss(t, users, pos, neg, off_u, off_i, w=None, distinct=False, keys=None
                          neg.to(torch.int64).contiguous(), off_u, off_i, distinct, keys)
 
 
+# ------------------------------------------------------------------ catalogue training and serving
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # IGR_DTYPE_*
+
+
+def _table(t, what):
+    """A 2-D float table with unit inner stride; returns (tensor, leading dim, IGR_DTYPE_*)."""
+    if t.dtype not in _DTYPES:
+        raise IgrError(f'{what}: expected float32, bfloat16 or float16, got {t.dtype}')
+    if t.dim() != 2:
+        raise IgrError(f'{what}: expected a 2-D tensor, got {tuple(t.shape)}')
+    if (t.stride(1) != 1 and t.shape[1] > 1) or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, max(t.stride(0), t.shape[1]), _DTYPES[t.dtype]
+
+
+def _same_device(*ts):
+    _dev(*ts)
+    dev = {t.device for t in ts if t is not None}
+    if len(dev) > 1:
+        raise IgrError(f'tensors on different devices: {sorted(map(str, dev))}')
+
+
+def _buffer(nbytes, device):
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+SOFTMAX_LOSS_MAX_WIDTH = 256
+
+
+class SoftmaxLoss(torch.autograd.Function):
+    """softmax_loss's node: the packed tables, the log-sums and the softmax-weighted item rows of the
+    forward are all that the backward needs besides one recomputation of the logits."""
+
+    @staticmethod
+    def forward(ctx, x, items, target, scale, ignore_index, reduction):
+        xs, ldx, dt = _table(x, 'softmax_loss x')
+        ws, ldw, _ = _table(items, 'softmax_loss items')
+        (B, d), V, dev = xs.shape, ws.shape[0], xs.device
+        need_x, need_w = ctx.needs_input_grad[:2]
+        lib = L.lib()
+        with torch.cuda.device(dev):
+            packs = [_buffer(lib.igr_softmax_loss_pack_size(n, d, dt), dev) for n in (B, V)]
+            loss, lse = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
+            total = count = o = None
+            if reduction != 'none':
+                total, count = torch.empty((), device=dev), torch.empty((), device=dev)
+            if need_x:
+                width = next(w for w in (32, 64, 128, 256) if w >= d)
+                o = torch.empty(B, width, dtype=torch.float32, device=dev)
+            wsb = lib.igr_softmax_loss_workspace_size(B, V, d, 0, int(need_x))
+            L.call('igr_softmax_loss_fwd', dt, B, V, d, _p(xs), ldx, _p(ws), ldw, _p(target), ignore_index, scale,
+                   int(reduction == 'mean'), _p(packs[0]), _p(packs[1]), _p(loss), _p(lse), _p(total), _p(count),
+                   _p(o), _p(_buffer(wsb, dev)), wsb, _stream())
+        if need_x or need_w:
+            ctx.save_for_backward(items, target, packs[0], packs[1], lse, count, o)
+            ctx.args = (dt, B, V, d, scale, ignore_index, reduction)
+        return loss if reduction == 'none' else total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        items, target, x_pack, w_pack, lse, count, o = ctx.saved_tensors
+        dt, B, V, d, scale, ignore_index, reduction = ctx.args
+        ws, ldw, _ = _table(items, 'softmax_loss items')
+        dev = ws.device
+        with torch.cuda.device(dev):
+            grad = _f32(grad).contiguous()
+            dx = torch.empty(B, d, dtype=ws.dtype, device=dev) if ctx.needs_input_grad[0] else None
+            dw = None
+            if ctx.needs_input_grad[1]:
+                dw = (torch.empty if B else torch.zeros)(V, d, dtype=ws.dtype, device=dev)
+            wsb = L.lib().igr_softmax_loss_workspace_size(B, V, d, 1, 0)
+            L.call('igr_softmax_loss_bwd', dt, B, V, d, _p(ws), ldw, _p(target), ignore_index, scale,
+                   int(reduction == 'mean'), int(reduction == 'none'), _p(grad), _p(x_pack), _p(w_pack), _p(lse),
+                   _p(count), _p(o), _p(dx), _p(dw), _p(_buffer(wsb, dev)), wsb, _stream())
+        return dx, dw, None, None, None, None
+
+
+def softmax_loss(x, items, target, scale=1.0, ignore_index=-100, reduction='mean'):
+    """Softmax cross entropy of batch rows x [B, d] against the whole item table items [V, d], without the
+    [B, V] logits in memory, with the gradients of both tables:
+        loss_b = log sum_v exp(scale <x_b, items_v>) - scale <x_b, items_target(b)>
+    (the full-catalogue form of the sampled BPR loss; scale = 1 / temperature).  x and items
+    share one type: float32, bfloat16 or float16; d <= SOFTMAX_LOSS_MAX_WIDTH.  Rows whose target
+    is ignore_index count for nothing, whatever they hold.  reduction 'mean' (over the other
+    rows; 0 if there are none), 'sum' or 'none' ([B]); the loss is float32.  A target outside
+    the table makes its row's loss, and every gradient it enters, NaN (no host check)."""
+    _same_device(x, items, target)
+    if reduction not in ('mean', 'sum', 'none'):
+        raise IgrError(f'softmax_loss: reduction {reduction!r}')
+    if x.dim() != 2 or items.dim() != 2 or target.dim() != 1 or x.shape[1] != items.shape[1] or \
+            target.shape[0] != x.shape[0]:
+        raise IgrError(f'softmax_loss shapes: x {tuple(x.shape)}, items {tuple(items.shape)}, target '
+                       f'{tuple(target.shape)}')
+    if x.dtype != items.dtype or x.dtype not in _DTYPES:
+        raise IgrError(f'softmax_loss: x {x.dtype} and items {items.dtype} must share float32, bfloat16 or float16')
+    if target.dtype not in (torch.int64, torch.int32):
+        raise IgrError(f'softmax_loss: target must be int64 or int32, got {target.dtype}')
+    if not 1 <= x.shape[1] <= SOFTMAX_LOSS_MAX_WIDTH:
+        raise IgrError(f'softmax_loss: width {x.shape[1]} outside 1..{SOFTMAX_LOSS_MAX_WIDTH}')
+    if items.shape[0] == 0:
+        raise IgrError('softmax_loss: no items')
+    if not (scale > 0 and math.isfinite(scale)):
+        raise IgrError(f'softmax_loss: scale must be positive and finite, got {scale}')
+    return SoftmaxLoss.apply(x, items, target.to(torch.int64).contiguous(), float(scale), int(ignore_index), reduction)
+
+
 # ------------------------------------------------------------------ DGL-compatible API
 
 def graph(edges, num_nodes=None, device='cuda'):

@@ -1,0 +1,55 @@
+"""Argument checks of the catalogue operators that are made before any GPU work (CPU)."""
+import ctypes
+
+import pytest
+import torch
+
+from igr import _lib as L
+from igr import ops
+
+
+def test_softmax_loss_refuses_cpu_tensors():
+    with pytest.raises(L.IgrError, match='no CPU fallback'):
+        ops.softmax_loss(torch.zeros(2, 4), torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64))
+
+
+def test_softmax_loss_c_arguments():
+    lib = L.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 255) & ~255
+
+    def fwd(dtype=0, b=4, v=6, d=8, ldx=8, ldw=8, scale=1.0, x=p, ws=p, wsb=1 << 40, total=p, count=p):
+        return lib.igr_softmax_loss_fwd(dtype, b, v, d, x, ldx, p, ldw, p, -100, scale, 1, p, p, p, p, total, count, None,
+                                        ws, wsb, None)
+
+    for kw, msg in ((dict(dtype=3), 'dtype'), (dict(b=-1), 'sizes'), (dict(v=0), 'sizes'), (dict(d=0), 'sizes'),
+                    (dict(v=1 << 31), 'rows'), (dict(ldx=7), 'leading'), (dict(ldw=7), 'leading'),
+                    (dict(scale=0.0), 'scale'), (dict(scale=float('nan')), 'scale'), (dict(x=None), 'null'),
+                    (dict(ws=None), 'workspace'), (dict(wsb=16), 'workspace'), (dict(ws=p + 4), 'workspace'),
+                    (dict(count=None), 'together')):
+        assert fwd(**kw) == 1, kw  # IGR_ERR_ARG
+        assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
+    assert fwd(d=257, ldx=257, ldw=257) == 3  # IGR_ERR_UNSUPPORTED
+
+    def bwd(dtype=0, d=8, ldw=8, scale=1.0, grad=p, ws=p, wsb=1 << 40, count=p):
+        return lib.igr_softmax_loss_bwd(dtype, 4, 6, d, p, ldw, p, -100, scale, 1, 0, grad, p, p, p, count, p, p, p, ws, wsb,
+                                        None)
+
+    for kw, msg in ((dict(dtype=-1), 'dtype'), (dict(ldw=7), 'leading'), (dict(scale=-1.0), 'scale'),
+                    (dict(grad=None), 'null'), (dict(count=None), 'null'), (dict(ws=None), 'workspace'),
+                    (dict(wsb=16), 'workspace')):
+        assert bwd(**kw) == 1, kw
+        assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
+
+
+def test_softmax_loss_sizes():
+    lib = L.lib()
+    # two 16-bit planes in two layouts for fp32, one plane for half types, an exponent a block of 32
+    assert lib.igr_softmax_loss_pack_size(64, 64, 0) == 2 * (2 * 2 * 32 * 64 * 2) + 256
+    assert lib.igr_softmax_loss_pack_size(33, 33, 1) == 2 * (2 * 32 * 64 * 2) + 256
+    assert lib.igr_softmax_loss_pack_size(0, 64, 0) == 0 and lib.igr_softmax_loss_pack_size(4, 300, 0) == 0
+    for b, v, d in ((1, 1, 1), (2048, 1000000, 64), (1, 1000000, 256), (100000, 7, 128)):
+        for back in (0, 1):
+            ws = lib.igr_softmax_loss_workspace_size(b, v, d, back, 1)
+            # partials of at most 512 workgroups of 256 rows, rounded up, and the rows' own data
+            assert 0 < ws <= 4 * (512 + 256) * 256 * (256 + 4) + 16 * (b + 512 * 32) + 4096 + 8 * 256 * min(b, v), (b, v, ws)
