@@ -567,6 +567,24 @@ int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const v
                          const float *count, const float *o, void *dx, void *dw, void *workspace,
                          int64_t ws_bytes, void *stream);
 
+/* ------------------------------------------------------- 8-bit serving */
+
+/* Rows to 8 bits with a scale each: a_r = max_k |x_rk|, q_rk = rint(x_rk / a_r * 127) (32-bit
+ * arithmetic, ties to even), scale_r = a_r / 127.  A row of zeros has q = 0 and scale 0; one
+ * that holds an infinity or NaN q = 0 and scale NaN.  x [n, k] of `dtype` (IGR_DTYPE_*), any alignment;
+ * q [n, ldq]: columns k..ldq are set to 0. */
+int igr_quantize_rows(int32_t dtype, int64_t n, int32_t k, const void *x, int64_t ldx, int8_t *q, int64_t ldq,
+                      float *scale, void *stream);
+
+/* c[m, n] = (sum_k a[m, k] b[n, k]) a_scale[m] b_scale[n], c of `out_dtype`: the scores of quantised
+ * users against quantised items.  The sums are exact (32-bit integers, k <= 131071); one
+ * rounding of the sum to fp32, one for each scale, one to the output type.  Any strides >= k (>= n)
+ * and any alignment (of c: its element's); nothing outside the given rows and columns is
+ * read or written. */
+int igr_gemm_int8(int64_t m, int64_t n, int32_t k, const int8_t *a, int64_t lda, const float *a_scale,
+                  const int8_t *b, int64_t ldb, const float *b_scale, int32_t out_dtype, void *c, int64_t ldc,
+                  void *stream);
+
 #ifdef __cplusplus
 }
 #endif

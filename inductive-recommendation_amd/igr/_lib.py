@@ -132,6 +132,9 @@ SIGNATURES = {
                                             c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
     'igr_softmax_loss_bwd': (ctypes.c_int, [c_i32, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_f32, c_i32, c_i32,
                                             c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    'igr_quantize_rows': (ctypes.c_int, [c_i32, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    'igr_gemm_int8': (ctypes.c_int, [c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i32, c_vp, c_i64,
+                                     c_vp]),
     'igr_loss_combine_f32': (ctypes.c_int, [c_vp, c_vp, c_vp, c_f32, c_f32, c_f32, c_vp, c_vp, c_vp]),
 }
 

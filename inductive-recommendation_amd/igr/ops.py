@@ -1306,6 +1306,55 @@ def softmax_loss(x, items, target, scale=1.0, ignore_index=-100, reduction='mean
     return SoftmaxLoss.apply(x, items, target.to(torch.int64).contiguous(), float(scale), int(ignore_index), reduction)
 
 
+def quantize_rows(x):
+    """(q, scale): each row of x [n, k] (float32, bfloat16 or float16) in 8 bits, q = rint(x / max|row| * 127) and
+    scale = max|row| / 127, so x ~ q * scale[:, None] within half a step.  A row of zeros has scale
+    0; a row that holds an infinity or NaN has q = 0 and scale NaN, which its products show.  q's rows are
+    stored 16-byte aligned (a view of a wider buffer where 16 does not divide k).  No gradient."""
+    _dev(x)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise IgrError(f'quantize_rows: expected a 2-D tensor with columns, got {tuple(x.shape)}')
+    xs, ldx, dt = _table(x.detach(), 'quantize_rows')
+    n, k = xs.shape
+    ldq = (k + 15) // 16 * 16
+    with torch.cuda.device(xs.device):
+        q = torch.empty(n, ldq, dtype=torch.int8, device=xs.device)
+        scale = torch.empty(n, dtype=torch.float32, device=xs.device)
+        L.call('igr_quantize_rows', dt, n, k, _p(xs), ldx, _p(q), ldq, _p(scale), _stream())
+    return q[:, :k], scale
+
+
+def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):
+    """Scores [m, n] = (a b^T) * a_scale[:, None] * b_scale[None, :] of two quantised tables (quantize_rows):
+    a [m, k] and b [n, k] int8, one float32 scale per row (token) of a and per row (channel) of b.  The
+    sums are exact; out_dtype float32, bfloat16 or float16.  No gradient."""
+    _same_device(a, a_scale, b, b_scale)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise IgrError(f'gemm_int8: expected int8 tables, got {a.dtype} and {b.dtype}')
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[1]:
+        raise IgrError(f'gemm_int8 shapes: {tuple(a.shape)} and {tuple(b.shape)}')
+    if out_dtype not in _DTYPES:
+        raise IgrError(f'gemm_int8: out_dtype {out_dtype}')
+    (m, k), n = a.shape, b.shape[0]
+    for s, r in ((a_scale, m), (b_scale, n)):
+        if _f32(s).shape != (r,):
+            raise IgrError(f'gemm_int8: scales {tuple(s.shape)} for {r} rows')
+    if not 1 <= k <= 131071:
+        raise IgrError(f'gemm_int8: k = {k} outside 1..131071')
+
+    def rows(t):
+        if (t.stride(1) != 1 and k > 1) or t.stride(0) < k:
+            t = t.contiguous()
+        return t, max(t.stride(0), k)
+    a, lda = rows(a)
+    b, ldb = rows(b)
+    with torch.cuda.device(a.device):
+        c = torch.empty(m, n, dtype=out_dtype, device=a.device)
+        L.call('igr_gemm_int8', m, n, k, _p(a), lda, _p(a_scale.contiguous()), _p(b), ldb, _p(b_scale.contiguous()),
+               _DTYPES[out_dtype], _p(c), n, _stream())
+    return c
+
+
 # ------------------------------------------------------------------ DGL-compatible API
 
 def graph(edges, num_nodes=None, device='cuda'):

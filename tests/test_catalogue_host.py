@@ -53,3 +53,31 @@ def test_softmax_loss_sizes():
             ws = lib.igr_softmax_loss_workspace_size(b, v, d, back, 1)
             # partials of at most 512 workgroups of 256 rows, rounded up, and the rows' own data
             assert 0 < ws <= 4 * (512 + 256) * 256 * (256 + 4) + 16 * (b + 512 * 32) + 4096 + 8 * 256 * min(b, v), (b, v, ws)
+
+
+def test_int8_refuses_cpu_tensors():
+    with pytest.raises(L.IgrError, match='no CPU fallback'):
+        ops.quantize_rows(torch.zeros(2, 4))
+    q, s = torch.zeros(2, 4, dtype=torch.int8), torch.ones(2)
+    with pytest.raises(L.IgrError, match='no CPU fallback'):
+        ops.gemm_int8(q, s, q, s)
+
+
+def test_int8_c_arguments():
+    lib = L.lib()
+
+    def quant(dtype=0, n=2, k=8, x=4096, ldx=8, q=4096, ldq=16, s=4096):
+        return lib.igr_quantize_rows(dtype, n, k, x, ldx, q, ldq, s, None)
+
+    def mul(m=2, n=3, k=8, a=4096, lda=8, sa=4096, ldb=8, out=0, c=4096, ldc=3):
+        return lib.igr_gemm_int8(m, n, k, a, lda, sa, 4096, ldb, 4096, out, c, ldc, None)
+
+    for f, kw, msg in ((quant, dict(dtype=7), 'dtype'), (quant, dict(n=-1), 'sizes'), (quant, dict(k=0), 'sizes'),
+                       (quant, dict(ldx=7), 'leading'), (quant, dict(ldq=7), 'leading'), (quant, dict(x=None), 'null'),
+                       (quant, dict(q=None), 'null'), (quant, dict(s=None), 'null'), (mul, dict(out=3), 'dtype'),
+                       (mul, dict(m=-1), 'sizes'), (mul, dict(k=0), 'sizes'), (mul, dict(k=131072, lda=1 << 20), '131071'),
+                       (mul, dict(lda=7), 'leading'), (mul, dict(ldb=7), 'leading'), (mul, dict(ldc=2), 'leading'),
+                       (mul, dict(a=None), 'null'), (mul, dict(sa=None), 'null'), (mul, dict(c=None), 'null')):
+        assert f(**kw) == 1, kw
+        assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
+    assert quant(n=0) == 0 and mul(m=0) == 0 and mul(n=0, ldc=0) == 0  # nothing to do, no launch
