@@ -1,0 +1,576 @@
+// newton_schulz.hip - orthogonalising a weight's update by Newton-Schulz products (gfx950 matrix cores).
+//
+//   X_0 = G / (|G|_F + eps),   A = X X^T,   X <- a X + (b A + c A A) X        steps times
+// on the side with fewer rows (G^T for a tall G).  The iteration pushes X's singular values towards
+// 1 and amplifies the small ones by a each step, so its products need fp32's accuracy: every matrix
+// is held as pairs of halves (half_split.h) and multiplied in three 16-bit products.  X's
+// singular values stay below about 1.2 and A's and b A + c A A's entries below 3, so one
+// fixed scale 2^11 serves all of them: entries up to 32, down to steps of 2^-35.
+//
+// A and Q = b A + c A A are symmetric: only tiles on and below the diagonal are computed.
+//
+// A matrix is kept as MFMA fragments (32 rows x 16 columns, 64 lanes of 16 bytes, two planes), so a tile
+// is loaded as it lies.  A product needs both operands along the contraction: X as rows (for A) and X^T as
+// rows (for Q X), which the update writes together, one straight from the MFMA layout (a
+// lane holds four consecutive rows of a column), the other turned in LDS.
+//
+// Small matrices (up to 64 x 256, a recommender's dense layers) run all steps in one workgroup, X in
+// LDS: a launch each is what they would cost otherwise.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "half_split.h"
+
+namespace igr {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kScale = 11;
+typedef Frags<SplitF32> Frag2;
+
+struct Mat {  // a strided batch of matrices, oriented so that rows <= cols: element (r, c) at r sr + c sc
+    int64_t S, L, sr, sc, sb;
+};
+
+__device__ __forceinline__ void load2(const uint4 *p, int64_t frag, int lane, Frag2 &f) {
+    f.p[0] = __builtin_bit_cast(half8_t, p[(frag * 2) * 64 + lane]);
+    f.p[1] = __builtin_bit_cast(half8_t, p[(frag * 2 + 1) * 64 + lane]);
+}
+
+// Four values as (hi, lo) halves.
+struct Quad {
+    uint2 hi, lo;
+};
+__device__ __forceinline__ Quad split4(float a, float b, float c, float d) {
+    const half2_t h0 = __builtin_convertvector((float2_t{a, b}), half2_t);
+    const half2_t h1 = __builtin_convertvector((float2_t{c, d}), half2_t);
+    const half2_t l0 = __builtin_convertvector((float2_t{rest_of<0>(h0, a), rest_of<1>(h0, b)}), half2_t);
+    const half2_t l1 = __builtin_convertvector((float2_t{rest_of<0>(h1, c), rest_of<1>(h1, d)}), half2_t);
+    return {make_uint2(__builtin_bit_cast(uint32_t, h0), __builtin_bit_cast(uint32_t, h1)),
+            make_uint2(__builtin_bit_cast(uint32_t, l0), __builtin_bit_cast(uint32_t, l1))};
+}
+__device__ __forceinline__ float half_at(uint2 v, int i) {
+    const uint32_t w = i < 2 ? v.x : v.y;
+    return (float)__builtin_bit_cast(half2_t, w)[i & 1];
+}
+
+// A 32 x 32 result block (lane: column n % 32, register 4 g + i: row 8 g + 4 h + i) as part of a
+// fragment matrix whose rows are the block's columns: 8 bytes a group of four rows.
+__device__ __forceinline__ int64_t quad_index(int64_t row_block, int64_t KS, int64_t k0, int g, int lane, int plane) {
+    const int64_t frag = row_block * KS + (k0 >> 4) + (g >> 1);
+    return ((frag * 2 + plane) * 64 + (lane & 31) + 32 * (g & 1)) * 2 + (lane >> 5);
+}
+__device__ __forceinline__ void put_block(uint4 *dst, int64_t row_block, int64_t KS, int64_t k0,
+                                          const float (&v)[16], int lane) {
+    uint2 *d = reinterpret_cast<uint2 *>(dst);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const Quad q = split4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        d[quad_index(row_block, KS, k0, g, lane, 0)] = q.hi;
+        d[quad_index(row_block, KS, k0, g, lane, 1)] = q.lo;
+    }
+}
+__device__ __forceinline__ void get_block(const uint4 *src, int64_t row_block, int64_t KS, int64_t k0, float (&v)[16],
+                                          int lane) {
+    const uint2 *s = reinterpret_cast<const uint2 *>(src);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const uint2 hi = s[quad_index(row_block, KS, k0, g, lane, 0)];
+        const uint2 lo = s[quad_index(row_block, KS, k0, g, lane, 1)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * g + i] = half_at(hi, i) + half_at(lo, i);
+    }
+}
+
+// ------------------------------------------------------------------ one workgroup a matrix
+
+// X: 64 x 64 NW in two blocks of rows and 2 NW of columns; wave w holds row block w & 1 of column
+// blocks (w >> 1) + 2 j in registers, in fp32, and block (w >> 1, w & 1) of A.
+template <class T, int NW>
+__global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g, T *y, int32_t steps, float ca,
+                                                     float cb, float cc, double eps) {
+    constexpr int KL = 4 * NW;  // 16-column steps of X's rows
+    __shared__ uint4 xs[2 * KL * 2 * 64], xt[2 * NW * 4 * 2 * 64], am[2 * 4 * 2 * 64], qm[2 * 4 * 2 * 64];
+    double *red = reinterpret_cast<double *>(qm);  // qm is first written two barriers later
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
+    const int mb = wave & 1, nb0 = wave >> 1;
+    const T *src = g + blockIdx.x * in.sb;
+    float x[NW][16];
+    double ss = 0.;
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = mb * 32 + 8 * (i >> 2) + 4 * h + (i & 3), c = (nb0 + 2 * j) * 32 + col;
+            x[j][i] = r < in.S && c < in.L ? (float)src[r * in.sr + c * in.sc] : 0.f;
+            ss += (double)x[j][i] * x[j][i];
+        }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if (lane == 0) red[wave] = ss;
+    __syncthreads();
+    const double inv = 1. / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
+    constexpr float up = 1 << kScale, down = 1.f / (1 << kScale);
+    // values in x are X 2^11, as the fragments hold them
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[j][i] = (float)(x[j][i] * inv) * up;
+
+    auto store_x = [&]() {
+        _Float16 *rows = reinterpret_cast<_Float16 *>(xs);
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+            const int nb = nb0 + 2 * j;
+            put_block(xt, nb, 4, mb * 32, x[j], lane);
+            // the rows' fragments: this lane's column is one half of 16 different lanes' 16 bytes
+            const int at = ((mb * KL + nb * 2 + (col >> 4)) * 2 * 64 + 32 * ((col >> 3) & 1)) * 8 + (col & 7);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int r = 8 * (i >> 2) + 4 * h + (i & 3);
+                const _Float16 hi = (_Float16)x[j][i];
+                rows[at + r * 8] = hi;
+                rows[at + r * 8 + 64 * 8] = (_Float16)(x[j][i] - (float)hi);
+            }
+        }
+    };
+    store_x();
+    __syncthreads();
+    for (int s = 0; s < steps; ++s) {
+        f32x16_t acc;
+        float av[16], v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < KL; ++k) {
+            Frag2 p, q;
+            load2(xs, nb0 * KL + k, lane, p);
+            load2(xs, mb * KL + k, lane, q);
+            acc = mfma_split<SplitF32>(p, q, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) av[i] = acc[i] * down;
+        put_block(am, mb, 4, nb0 * 32, av, lane);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            Frag2 p, q;
+            load2(am, nb0 * 4 + k, lane, p);
+            load2(am, mb * 4 + k, lane, q);
+            acc = mfma_split<SplitF32>(p, q, acc);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = fmaf(cb, av[i], cc * (acc[i] * down));
+        put_block(qm, mb, 4, nb0 * 32, v, lane);
+        __syncthreads();
+        Frag2 qf[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) load2(qm, mb * 4 + k, lane, qf[k]);
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                Frag2 q;
+                load2(xt, (nb0 + 2 * j) * 4 + k, lane, q);
+                acc = mfma_split<SplitF32>(qf[k], q, acc);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[j][i] = fmaf(ca, x[j][i], acc[i] * down);
+        }
+        if (s + 1 < steps) {
+            __syncthreads();
+            store_x();
+            __syncthreads();
+        }
+    }
+    T *dst = y + blockIdx.x * out.sb;
+#pragma unroll
+    for (int j = 0; j < NW; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = mb * 32 + 8 * (i >> 2) + 4 * h + (i & 3), c = (nb0 + 2 * j) * 32 + col;
+            if (r < out.S && c < out.L) dst[r * out.sr + c * out.sc] = (T)(x[j][i] * down);
+        }
+}
+
+// ------------------------------------------------------------------ tiles over the whole chip
+
+constexpr int kSumBlocks = 64;  // partial sums of squares a matrix
+
+template <class T>
+__global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double *part) {
+    __shared__ double red[4];
+    const T *src = g + (int64_t)blockIdx.y * in.sb;
+    // the unit-stride side is walked by the threads
+    const bool flip = in.sr == 1;
+    const int64_t rows = flip ? in.L : in.S, cols = flip ? in.S : in.L, ld = flip ? in.sc : in.sr;
+    double s = 0.;
+    const int64_t n = rows * cols, step = (int64_t)gridDim.x * kThreads;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
+        const float v = (float)src[i / cols * ld + i % cols];
+        s += (double)v * v;
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.y * kSumBlocks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+struct Work {  // fragment matrices of one matrix of the batch; the next one's follow at the strides
+    uint4 *x, *xt[2], *a, *q;
+    int64_t bx, ba;    // strides between matrices, in uint4
+    int64_t Sp, Lp;    // padded sides, multiples of the tile
+};
+
+// 32 x 32 blocks of X_0 into both fragment matrices, zeros in the padding.
+template <class T>
+__global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const double *part, double eps, Work w) {
+    __shared__ float tile[4][32][33];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int64_t batch = blockIdx.y, nb = w.Lp / 32, blocks = nb * (w.Sp / 32);
+    double ss = 0.;
+    for (int i = 0; i < kSumBlocks; ++i) ss += part[batch * kSumBlocks + i];  // the same order everywhere
+    const double inv = 1. / (sqrt(ss) + eps);
+    const T *src = g + batch * in.sb;
+    const int64_t blk = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t r0 = blk / nb * 32, c0 = blk % nb * 32;
+    const bool flip = in.sr == 1;
+    if (blk < blocks) {
+#pragma unroll 4
+        for (int i = lane; i < 1024; i += 64) {
+            const int r = flip ? i & 31 : i >> 5, c = flip ? i >> 5 : i & 31;
+            float v = 0.f;
+            if (r0 + r < in.S && c0 + c < in.L)
+                v = (float)((double)(float)src[(r0 + r) * in.sr + (c0 + c) * in.sc] * inv) * (float)(1 << kScale);
+            tile[wave][r][c] = v;
+        }
+    }
+    __syncthreads();
+    if (blk >= blocks) return;
+    const int row = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float a[8], b[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            a[e] = tile[wave][row][k * 16 + h * 8 + e];
+            b[e] = tile[wave][k * 16 + h * 8 + e][row];
+        }
+        Frag2 f;
+        split8(a, f);
+        uint4 *x = w.x + batch * w.bx + ((r0 / 32 * (w.Lp / 16) + c0 / 16 + k) * 2) * 64 + lane;
+        x[0] = __builtin_bit_cast(uint4, f.p[0]);
+        x[64] = __builtin_bit_cast(uint4, f.p[1]);
+        split8(b, f);
+        uint4 *xt = w.xt[0] + batch * w.bx + ((c0 / 32 * (w.Sp / 16) + r0 / 16 + k) * 2) * 64 + lane;
+        xt[0] = __builtin_bit_cast(uint4, f.p[0]);
+        xt[64] = __builtin_bit_cast(uint4, f.p[1]);
+    }
+}
+
+// The three products of a step (and the last one, into the caller's matrix).
+enum Mode { kGram, kPoly, kUpdate, kLast };
+
+struct Prod {
+    const uint4 *p, *q;     // fragment matrices: rows of the result, columns of the result
+    int64_t bp, bq;         // batch strides
+    int64_t KS;             // 16-column steps of both
+    int64_t tn;             // tiles along the columns (kUpdate, kLast)
+    uint4 *d0, *d1;         // result as rows = its columns (straight) and rows = its rows (turned)
+    int64_t KS0, KS1, b0, b1;
+    const uint4 *add;       // what is added, with d0's layout
+    int64_t badd;
+    float f_add, f_mul;     // result = f_add add + f_mul product
+};
+
+// One 32 x 32 block at (m0, n0): scaled, added to, written both ways.  `turn` is a wave's 32 x 33 floats.
+template <int MODE, class T>
+__device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_t batch, int64_t m0, int64_t n0,
+                                     bool mirror, const f32x16_t &acc, float (*turn)[33], int lane) {
+    constexpr float down = 1.f / (1 << kScale);
+    float v[16];
+    if constexpr (MODE == kGram) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = acc[i] * down;
+    } else {
+        get_block(a.add + batch * a.badd, n0 / 32, a.KS0, m0, v, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = fmaf(a.f_add, v[i], a.f_mul * (acc[i] * down));
+    }
+    if constexpr (MODE == kLast) {
+        T *dst = y + batch * out.sb;
+        const int64_t c = n0 + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = m0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+            if (r < out.S && c < out.L) dst[r * out.sr + c * out.sc] = (T)(v[i] * down);
+        }
+        return;
+    }
+    put_block(a.d0 + batch * a.b0, n0 / 32, a.KS0, m0, v, lane);
+    if (!mirror) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) turn[8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)][lane & 31] = v[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        float r[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e] = turn[lane & 31][k * 16 + 8 * (lane >> 5) + e];
+        Frag2 f;
+        split8(r, f);
+        uint4 *d = a.d1 + batch * a.b1 + ((m0 / 32 * a.KS1 + n0 / 16 + k) * 2) * 64 + lane;
+        d[0] = __builtin_bit_cast(uint4, f.p[0]);
+        d[64] = __builtin_bit_cast(uint4, f.p[1]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int MODE>
+__device__ __forceinline__ void tile_of(int64_t id, int64_t tn, int64_t &m, int64_t &n) {
+    if constexpr (MODE == kGram || MODE == kPoly) {  // tiles on and below the diagonal, row by row
+        m = (int64_t)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+        while (m * (m + 1) / 2 > id) --m;
+        while ((m + 1) * (m + 2) / 2 <= id) ++m;
+        n = id - m * (m + 1) / 2;
+    } else {
+        m = id / tn;
+        n = id % tn;
+    }
+}
+
+// Few tiles: 64 x 64 a workgroup, the contraction dealt out to its four waves, which load fragments straight
+// from memory and join their sums in LDS in wave order.
+template <int MODE, class T>
+__global__ __launch_bounds__(kThreads) void ns_prod64(Prod a, Mat out, T *y) {
+    __shared__ float part[4][4][16][64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int64_t batch = blockIdx.y;
+    int64_t tm, tn;
+    tile_of<MODE>(blockIdx.x, a.tn, tm, tn);
+    const uint4 *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
+    f32x16_t acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i >> 1][i & 1][r] = 0.f;
+    for (int64_t k = wave; k < a.KS; k += 4) {
+        Frag2 fp[2], fq[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            load2(p, (tm * 2 + i) * a.KS + k, lane, fp[i]);
+            load2(q, (tn * 2 + i) * a.KS + k, lane, fq[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = mfma_split<SplitF32>(fp[i >> 1], fq[i & 1], acc[i >> 1][i & 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[wave][i][r][lane] = acc[i >> 1][i & 1][r];
+    __syncthreads();
+    f32x16_t s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        s[r] = (part[0][wave][r][lane] + part[1][wave][r][lane]) + (part[2][wave][r][lane] + part[3][wave][r][lane]);
+    __syncthreads();
+    const bool mirror = MODE == kUpdate || tm != tn;
+    emit<MODE, T>(a, out, y, batch, (tm * 2 + (wave >> 1)) * 32, (tn * 2 + (wave & 1)) * 32, mirror, s,
+                  reinterpret_cast<float (*)[33]>(&part[wave][0][0][0]), lane);
+}
+
+// Many tiles: 128 x 128 a workgroup, four waves of 64 x 64, two 16-column steps at a time through
+// double-buffered LDS (one barrier each).
+template <int MODE, class T>
+__global__ __launch_bounds__(kThreads, 2) void ns_prod128(Prod a, Mat out, T *y) {
+    constexpr int ST = 4 * 2 * 2 * 64;  // uint4 a stage of one operand: 4 row blocks, 2 steps, 2 planes
+    __shared__ uint4 lds[2][2][ST];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
+    const int64_t batch = blockIdx.y;
+    int64_t tm, tn;
+    tile_of<MODE>(blockIdx.x, a.tn, tm, tn);
+    // thread t stages 16 bytes of each row block: 256 threads are the block's 2 steps of 2 planes
+    const uint4 *p = a.p + batch * a.bp + tm * 4 * a.KS * 128 + t, *q = a.q + batch * a.bq + tn * 4 * a.KS * 128 + t;
+    uint4 sp[4], sq[4];
+    auto fetch = [&](int64_t k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sp[i] = p[(i * a.KS + k) * 128];
+            sq[i] = q[(i * a.KS + k) * 128];
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lds[buf][0][i * 256 + t] = sp[i];
+            lds[buf][1][i * 256 + t] = sq[i];
+        }
+    };
+    f32x16_t acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i >> 1][i & 1][r] = 0.f;
+    fetch(0);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (int64_t k = 0; k < a.KS; k += 2, buf ^= 1) {
+        const bool more = k + 2 < a.KS;
+        if (more) fetch(k + 2);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            Frag2 fp[2], fq[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                load2(lds[buf][0], (wm * 2 + i) * 2 + s, lane, fp[i]);
+                load2(lds[buf][1], (wn * 2 + i) * 2 + s, lane, fq[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc[i >> 1][i & 1] = mfma_split<SplitF32>(fp[i >> 1], fq[i & 1], acc[i >> 1][i & 1]);
+        }
+        if (more) stage(buf ^ 1);
+        __syncthreads();
+    }
+    const bool mirror = MODE == kUpdate || tm != tn;
+    float(*turn)[33] = reinterpret_cast<float(*)[33]>(reinterpret_cast<float *>(&lds[0][0][0]) + wave * 32 * 33);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        emit<MODE, T>(a, out, y, batch, (tm * 4 + wm * 2 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32, mirror,
+                      acc[i >> 1][i & 1], turn, lane);
+}
+
+// ------------------------------------------------------------------ host side
+
+struct Plan {
+    bool small;
+    int tile;
+    int64_t Sp, Lp, xsz, asz, bytes;
+};
+
+inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+inline Plan plan_of(int64_t batch, int64_t S, int64_t L) {
+    Plan p{};
+    p.small = S <= 64 && L <= 256;
+    if (p.small) return p;
+    // 128-wide tiles once the update has enough of them for half the chip
+    const int64_t n128 = ((S + 127) / 128) * ((L + 127) / 128) * batch;
+    p.tile = n128 >= 128 ? 128 : 64;
+    p.Sp = up_to(S, p.tile);
+    p.Lp = up_to(L, p.tile);
+    p.xsz = p.Sp * p.Lp / 4;  // uint4: 4 bytes an element
+    p.asz = p.Sp * p.Sp / 4;
+    p.bytes = batch * (3 * p.xsz + 2 * p.asz) * 16 + batch * kSumBlocks * 8;
+    return p;
+}
+
+template <class T>
+int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const void *g, void *y, int32_t steps, float ca,
+        float cb, float cc, double eps, void *ws, hipStream_t st) {
+    const T *src = static_cast<const T *>(g);
+    T *dst = static_cast<T *>(y);
+    if (p.small) {
+        const dim3 gr((unsigned)batch), b(kThreads);
+        if (in.L <= 64) hipLaunchKernelGGL((ns_small<T, 1>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps);
+        else if (in.L <= 128) hipLaunchKernelGGL((ns_small<T, 2>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps);
+        else hipLaunchKernelGGL((ns_small<T, 4>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps);
+        return launch_status(fn);
+    }
+    Work w{};
+    uint4 *c = static_cast<uint4 *>(ws);
+    w.x = c, c += batch * p.xsz;
+    w.xt[0] = c, c += batch * p.xsz;
+    w.xt[1] = c, c += batch * p.xsz;
+    w.a = c, c += batch * p.asz;
+    w.q = c, c += batch * p.asz;
+    double *part = reinterpret_cast<double *>(c);
+    w.bx = p.xsz, w.ba = p.asz, w.Sp = p.Sp, w.Lp = p.Lp;
+    const unsigned nb = (unsigned)batch;
+    hipLaunchKernelGGL((ns_sumsq<T>), dim3(kSumBlocks, nb), dim3(kThreads), 0, st, in, src, part);
+    const int64_t blocks = (p.Sp / 32) * (p.Lp / 32);
+    hipLaunchKernelGGL((ns_pack<T>), dim3((unsigned)((blocks + 3) / 4), nb), dim3(kThreads), 0, st, in, src, part, eps, w);
+    const int64_t ts = p.Sp / p.tile, tl = p.Lp / p.tile;
+    const unsigned tri = (unsigned)(ts * (ts + 1) / 2), all = (unsigned)(ts * tl);
+    const int64_t ks = p.Sp / 16, kl = p.Lp / 16;
+    auto go = [&](auto mode, const Prod &a, unsigned n) {
+        constexpr int M = decltype(mode)::value;
+        if (p.tile == 128) hipLaunchKernelGGL((ns_prod128<M, T>), dim3(n, nb), dim3(kThreads), 0, st, a, out, dst);
+        else hipLaunchKernelGGL((ns_prod64<M, T>), dim3(n, nb), dim3(kThreads), 0, st, a, out, dst);
+    };
+    for (int32_t s = 0; s < steps; ++s) {
+        uint4 *cur = w.xt[s & 1], *nxt = w.xt[(s + 1) & 1];
+        go(std::integral_constant<int, kGram>(),
+           Prod{w.x, w.x, w.bx, w.bx, kl, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f}, tri);
+        go(std::integral_constant<int, kPoly>(),
+           Prod{w.a, w.a, w.ba, w.ba, ks, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc}, tri);
+        const Prod u{w.q, cur, w.ba, w.bx, ks, tl, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f};
+        if (s + 1 < steps) go(std::integral_constant<int, kUpdate>(), u, all);
+        else go(std::integral_constant<int, kLast>(), u, all);
+    }
+    return launch_status(fn);
+}
+
+// The iterates of every singular value in [0, 1]: the fixed scale holds X up to 4 and Q up to 16.
+inline bool coefficients_fit(int32_t steps, double a, double b, double c) {
+    for (int i = 0; i <= 2000; ++i) {
+        double x = (double)i / 2000;
+        for (int32_t s = 0; s < steps; ++s) {
+            const double l = x * x, q = b * l + c * l * l;
+            x = a * x + q * x;
+            if (!(std::fabs(x) <= 4.) || !(std::fabs(q) <= 16.)) return false;
+        }
+    }
+    return true;
+}
+
+}  // namespace
+}  // namespace igr
+
+using namespace igr;
+
+extern "C" int64_t igr_newton_schulz_workspace_size(int64_t batch, int64_t rows, int64_t cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    return plan_of(batch, std::min(rows, cols), std::max(rows, cols)).bytes;
+}
+
+extern "C" int igr_newton_schulz(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, const void *g, int64_t ldg,
+                                 int64_t stride_g, int32_t steps, double a, double b, double c, double eps, void *out,
+                                 void *workspace, int64_t ws_bytes, void *stream) {
+    return guarded("igr_newton_schulz", [&]() -> int {
+        const char *fn = "igr_newton_schulz";
+        if (dtype < kF32 || dtype > kF16) return arg_error(fn, "unknown dtype");
+        if (batch < 0 || rows < 0 || cols < 0) return arg_error(fn, "negative size");
+        if (ldg < cols || (batch > 1 && stride_g < 0)) return arg_error(fn, "leading dimension too small");
+        if (steps < 1 || steps > 100) return arg_error(fn, "steps outside 1..100");
+        if (!(eps >= 0.) || !std::isfinite(eps)) return arg_error(fn, "eps must be finite and not negative");
+        if (!coefficients_fit(steps, a, b, c))
+            return arg_error(fn, "the coefficients drive singular values out of the range that is held");
+        if (batch == 0 || rows == 0 || cols == 0) return IGR_OK;
+        if (batch > 65535 || rows > (1 << 24) || cols > (1 << 24) || std::min(rows, cols) > (1 << 15))
+            return arg_error(fn, "too large: at most 65535 matrices, sides of 2^24, the shorter 2^15");
+        const int64_t S = std::min(rows, cols), L = std::max(rows, cols);
+        const Plan p = plan_of(batch, S, L);
+        if (!p.small && p.Sp / 32 * (p.Lp / 32) / 4 > INT32_MAX) return arg_error(fn, "too many tiles");
+        if (!g || !out) return arg_error(fn, "null pointer");
+        if (p.bytes > 0 && (!workspace || ws_bytes < p.bytes || !aligned16(workspace)))
+            return arg_error(fn, "workspace too small or not 16-byte aligned");
+        const bool flip = rows > cols;
+        const Mat in{S, L, flip ? 1 : ldg, flip ? ldg : 1, stride_g};
+        const Mat to{S, L, flip ? 1 : cols, flip ? cols : 1, rows * cols};
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        const float fa = (float)a, fb = (float)b, fc = (float)c;
+        if (dtype == kF32) return run<float>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, workspace, st);
+        if (dtype == kBF16) return run<__bf16>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, workspace, st);
+        return run<_Float16>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, workspace, st);
+    });
+}

@@ -135,6 +135,9 @@ SIGNATURES = {
     'igr_quantize_rows': (ctypes.c_int, [c_i32, c_i64, c_i32, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp]),
     'igr_gemm_int8': (ctypes.c_int, [c_i64, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i32, c_vp, c_i64,
                                      c_vp]),
+    'igr_newton_schulz_workspace_size': (c_i64, [c_i64, c_i64, c_i64]),
+    'igr_newton_schulz': (ctypes.c_int, [c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i32, ctypes.c_double,
+                                         ctypes.c_double, ctypes.c_double, ctypes.c_double, c_vp, c_vp, c_i64, c_vp]),
     'igr_loss_combine_f32': (ctypes.c_int, [c_vp, c_vp, c_vp, c_f32, c_f32, c_f32, c_vp, c_vp, c_vp]),
 }
 

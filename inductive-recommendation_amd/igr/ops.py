@@ -1355,6 +1355,34 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):
     return c
 
 
+NEWTON_SCHULZ_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def newton_schulz(g, steps=5, coeffs=NEWTON_SCHULZ_COEFFS, eps=1e-7):
+    """Orthogonalise g [rows, cols] or [batch, rows, cols] (float32, bfloat16 or float16): X = g / (|g|_F + eps), then
+    `steps` times X <- a X + (b A + c A A) X with A = X X^T (of g^T for a tall g), which drives every
+    singular value towards 1.  Carried in float32 accuracy whatever the type; the result has g's
+    type.  Used by optim.Muon.  No gradient."""
+    _dev(g)
+    if g.dtype not in _DTYPES:
+        raise IgrError(f'newton_schulz: expected float32, bfloat16 or float16, got {g.dtype}')
+    if g.dim() not in (2, 3):
+        raise IgrError(f'newton_schulz: expected [rows, cols] or [batch, rows, cols], got {tuple(g.shape)}')
+    if len(coeffs) != 3:
+        raise IgrError('newton_schulz: three coefficients expected')
+    x = g.detach() if g.dim() == 3 else g.detach()[None]
+    b, r, c = x.shape
+    if (x.stride(2) != 1 and c > 1) or x.stride(1) < c or x.stride(0) < 0:
+        x = x.contiguous()
+    with torch.cuda.device(x.device):
+        out = torch.empty(b, r, c, dtype=x.dtype, device=x.device)
+        wsb = L.lib().igr_newton_schulz_workspace_size(b, r, c)
+        ws = _buffer(wsb, x.device) if wsb else None
+        L.call('igr_newton_schulz', _DTYPES[x.dtype], b, r, c, _p(x), max(x.stride(1), c), x.stride(0), int(steps),
+               *(float(v) for v in coeffs), float(eps), _p(out), _p(ws), wsb, _stream())
+    return out.view(g.shape)
+
+
 # ------------------------------------------------------------------ DGL-compatible API
 
 def graph(edges, num_nodes=None, device='cuda'):

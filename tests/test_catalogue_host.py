@@ -81,3 +81,29 @@ def test_int8_c_arguments():
         assert f(**kw) == 1, kw
         assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
     assert quant(n=0) == 0 and mul(m=0) == 0 and mul(n=0, ldc=0) == 0  # nothing to do, no launch
+
+
+def test_newton_schulz_refuses_cpu_tensors():
+    with pytest.raises(L.IgrError, match='no CPU fallback'):
+        ops.newton_schulz(torch.zeros(2, 4))
+
+
+def test_newton_schulz_c_arguments():
+    lib = L.lib()
+
+    def ns(dtype=0, batch=1, rows=100, cols=300, ldg=300, sg=0, steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, g=4096,
+           ws=4096, wsb=1 << 40):
+        return lib.igr_newton_schulz(dtype, batch, rows, cols, g, ldg, sg, steps, a, b, c, eps, 4096, ws, wsb, None)
+
+    nan = float('nan')
+    for kw, msg in ((dict(dtype=3), 'dtype'), (dict(batch=-1), 'size'), (dict(ldg=299), 'leading'),
+                    (dict(batch=2, sg=-1), 'leading'), (dict(steps=0), 'steps'), (dict(steps=101), 'steps'),
+                    (dict(eps=-1.0), 'eps'), (dict(eps=nan), 'eps'), (dict(a=nan), 'coefficients'),
+                    (dict(a=5.0, b=0.0, c=0.0), 'coefficients'), (dict(batch=65536), 'large'),
+                    (dict(rows=40000, cols=40000, ldg=40000), 'large'), (dict(g=None), 'null'),
+                    (dict(ws=None), 'workspace'), (dict(wsb=16), 'workspace'), (dict(ws=4100), 'workspace')):
+        assert ns(**kw) == 1, kw
+        assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
+    assert ns(batch=0) == 0 and ns(rows=0) == 0
+    assert lib.igr_newton_schulz_workspace_size(6, 64, 64) == 0  # one workgroup a matrix
+    assert lib.igr_newton_schulz_workspace_size(1, 128, 512) == (3 * 128 * 512 + 2 * 128 * 128) * 4 + 64 * 8
