@@ -14,6 +14,7 @@
 
 namespace igr {
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));  // 16 bytes that a register array may hold
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -63,6 +64,20 @@ __device__ __forceinline__ int block_exponent(float amax) {
     return e < -100 ? -100 : e;
 }
 
+// N 16-byte groups from memory to LDS without passing through registers, `t` of 256 threads; complete after
+// copies_done().  (N a multiple of 64: a wave copies 1 KB as it lies.)
+template <int N>
+__device__ __forceinline__ void copy_to_lds(const u32x4_t *src, u32x4_t *dst, int t) {
+    static_assert(N % 64 == 0, "whole waves");
+    typedef const __attribute__((address_space(1))) u32x4_t *gptr;
+    typedef __attribute__((address_space(3))) u32x4_t *lptr;
+#pragma unroll
+    for (int i = 0; i < N; i += 256)
+        if (N % 256 == 0 || i + (t & ~63) < N)
+            __builtin_amdgcn_global_load_lds((gptr)(src + i + t), (lptr)(dst + i + (t & ~63)), 16, 0, 0);
+}
+__device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
+
 // Eight fp32 values as the NS fragments of one lane.
 template <class P>
 struct Frags {
@@ -111,6 +126,20 @@ __device__ __forceinline__ f32x16_t mfma_split(const Frags<P> &a, const Frags<P>
         c = mfma32(a.p[1], b.p[0], c);
     }
     return mfma32(a.p[0], b.p[0], c);
+}
+
+// acc[n] += a b[n]: the products of one a with NB b's, one part of all of them after the other, so
+// that consecutive MFMAs do not wait for each other's sums.
+template <class P, int NB, class B>
+__device__ __forceinline__ void mfma_row(const Frags<P> &a, const B &b, f32x16_t (&acc)[NB]) {
+    if constexpr (P::NS == 2) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[n] = mfma32(a.p[0], b(n).p[1], acc[n]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[n] = mfma32(a.p[1], b(n).p[0], acc[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[n] = mfma32(a.p[0], b(n).p[0], acc[n]);
 }
 
 #endif

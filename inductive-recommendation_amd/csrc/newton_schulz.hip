@@ -33,7 +33,7 @@ struct Mat {  // a strided batch of matrices, oriented so that rows <= cols: ele
     int64_t S, L, sr, sc, sb;
 };
 
-__device__ __forceinline__ void load2(const uint4 *p, int64_t frag, int lane, Frag2 &f) {
+__device__ __forceinline__ void load2(const u32x4_t *p, int64_t frag, int lane, Frag2 &f) {
     f.p[0] = __builtin_bit_cast(half8_t, p[(frag * 2) * 64 + lane]);
     f.p[1] = __builtin_bit_cast(half8_t, p[(frag * 2 + 1) * 64 + lane]);
 }
@@ -61,7 +61,7 @@ __device__ __forceinline__ int64_t quad_index(int64_t row_block, int64_t KS, int
     const int64_t frag = row_block * KS + (k0 >> 4) + (g >> 1);
     return ((frag * 2 + plane) * 64 + (lane & 31) + 32 * (g & 1)) * 2 + (lane >> 5);
 }
-__device__ __forceinline__ void put_block(uint4 *dst, int64_t row_block, int64_t KS, int64_t k0,
+__device__ __forceinline__ void put_block(u32x4_t *dst, int64_t row_block, int64_t KS, int64_t k0,
                                           const float (&v)[16], int lane) {
     uint2 *d = reinterpret_cast<uint2 *>(dst);
 #pragma unroll
@@ -71,7 +71,7 @@ __device__ __forceinline__ void put_block(uint4 *dst, int64_t row_block, int64_t
         d[quad_index(row_block, KS, k0, g, lane, 1)] = q.lo;
     }
 }
-__device__ __forceinline__ void get_block(const uint4 *src, int64_t row_block, int64_t KS, int64_t k0, float (&v)[16],
+__device__ __forceinline__ void get_block(const u32x4_t *src, int64_t row_block, int64_t KS, int64_t k0, float (&v)[16],
                                           int lane) {
     const uint2 *s = reinterpret_cast<const uint2 *>(src);
 #pragma unroll
@@ -91,7 +91,7 @@ template <class T, int NW>
 __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g, T *y, int32_t steps, float ca,
                                                      float cb, float cc, double eps) {
     constexpr int KL = 4 * NW;  // 16-column steps of X's rows
-    __shared__ uint4 xs[2 * KL * 2 * 64], xt[2 * NW * 4 * 2 * 64], am[2 * 4 * 2 * 64], qm[2 * 4 * 2 * 64];
+    __shared__ u32x4_t xs[2 * KL * 2 * 64], xt[2 * NW * 4 * 2 * 64], am[2 * 4 * 2 * 64], qm[2 * 4 * 2 * 64];
     double *red = reinterpret_cast<double *>(qm);  // qm is first written two barriers later
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
     const int mb = wave & 1, nb0 = wave >> 1;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
 
 // ------------------------------------------------------------------ tiles over the whole chip
 
-constexpr int kSumBlocks = 64;  // partial sums of squares a matrix
+constexpr int kSumBlocks = 256;  // partial sums of squares a matrix
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double *part) {
@@ -209,12 +209,15 @@ __global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double 
     // the unit-stride side is walked by the threads
     const bool flip = in.sr == 1;
     const int64_t rows = flip ? in.L : in.S, cols = flip ? in.S : in.L, ld = flip ? in.sc : in.sr;
+    int wide = 256;  // threads along a row
+    while (wide > 1 && wide / 2 >= cols) wide >>= 1;
+    const int t = threadIdx.x, across = kThreads / wide;
     double s = 0.;
-    const int64_t n = rows * cols, step = (int64_t)gridDim.x * kThreads;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += step) {
-        const float v = (float)src[i / cols * ld + i % cols];
-        s += (double)v * v;
-    }
+    for (int64_t r = (int64_t)blockIdx.x * across + t / wide; r < rows; r += (int64_t)gridDim.x * across)
+        for (int64_t c = t % wide; c < cols; c += wide) {
+            const float v = (float)src[r * ld + c];
+            s += (double)v * v;
+        }
 #pragma unroll
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -223,8 +226,8 @@ __global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double 
 }
 
 struct Work {  // fragment matrices of one matrix of the batch; the next one's follow at the strides
-    uint4 *x, *xt[2], *a, *q;
-    int64_t bx, ba;    // strides between matrices, in uint4
+    u32x4_t *x, *xt[2], *a, *q;
+    int64_t bx, ba;    // strides between matrices, in u32x4_t
     int64_t Sp, Lp;    // padded sides, multiples of the tile
 };
 
@@ -232,10 +235,16 @@ struct Work {  // fragment matrices of one matrix of the batch; the next one's f
 template <class T>
 __global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const double *part, double eps, Work w) {
     __shared__ float tile[4][32][33];
+    __shared__ double red[4];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int64_t batch = blockIdx.y, nb = w.Lp / 32, blocks = nb * (w.Sp / 32);
-    double ss = 0.;
-    for (int i = 0; i < kSumBlocks; ++i) ss += part[batch * kSumBlocks + i];  // the same order everywhere
+    static_assert(kSumBlocks == kThreads, "one partial sum a thread");
+    double ss = part[batch * kSumBlocks + t];  // joined in the same order by every workgroup
+#pragma unroll
+    for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if (lane == 0) red[wave] = ss;
+    __syncthreads();
+    ss = (red[0] + red[1]) + (red[2] + red[3]);
     const double inv = 1. / (sqrt(ss) + eps);
     const T *src = g + batch * in.sb;
     const int64_t blk = (int64_t)blockIdx.x * 4 + wave;
@@ -264,13 +273,13 @@ __global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const do
         }
         Frag2 f;
         split8(a, f);
-        uint4 *x = w.x + batch * w.bx + ((r0 / 32 * (w.Lp / 16) + c0 / 16 + k) * 2) * 64 + lane;
-        x[0] = __builtin_bit_cast(uint4, f.p[0]);
-        x[64] = __builtin_bit_cast(uint4, f.p[1]);
+        u32x4_t *x = w.x + batch * w.bx + ((r0 / 32 * (w.Lp / 16) + c0 / 16 + k) * 2) * 64 + lane;
+        x[0] = __builtin_bit_cast(u32x4_t, f.p[0]);
+        x[64] = __builtin_bit_cast(u32x4_t, f.p[1]);
         split8(b, f);
-        uint4 *xt = w.xt[0] + batch * w.bx + ((c0 / 32 * (w.Sp / 16) + r0 / 16 + k) * 2) * 64 + lane;
-        xt[0] = __builtin_bit_cast(uint4, f.p[0]);
-        xt[64] = __builtin_bit_cast(uint4, f.p[1]);
+        u32x4_t *xt = w.xt[0] + batch * w.bx + ((c0 / 32 * (w.Sp / 16) + r0 / 16 + k) * 2) * 64 + lane;
+        xt[0] = __builtin_bit_cast(u32x4_t, f.p[0]);
+        xt[64] = __builtin_bit_cast(u32x4_t, f.p[1]);
     }
 }
 
@@ -278,13 +287,13 @@ __global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const do
 enum Mode { kGram, kPoly, kUpdate, kLast };
 
 struct Prod {
-    const uint4 *p, *q;     // fragment matrices: rows of the result, columns of the result
+    const u32x4_t *p, *q;     // fragment matrices: rows of the result, columns of the result
     int64_t bp, bq;         // batch strides
     int64_t KS;             // 16-column steps of both
     int64_t tn;             // tiles along the columns (kUpdate, kLast)
-    uint4 *d0, *d1;         // result as rows = its columns (straight) and rows = its rows (turned)
+    u32x4_t *d0, *d1;         // result as rows = its columns (straight) and rows = its rows (turned)
     int64_t KS0, KS1, b0, b1;
-    const uint4 *add;       // what is added, with d0's layout
+    const u32x4_t *add;       // what is added, with d0's layout
     int64_t badd;
     float f_add, f_mul;     // result = f_add add + f_mul product
 };
@@ -326,9 +335,9 @@ __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_
         for (int e = 0; e < 8; ++e) r[e] = turn[lane & 31][k * 16 + 8 * (lane >> 5) + e];
         Frag2 f;
         split8(r, f);
-        uint4 *d = a.d1 + batch * a.b1 + ((m0 / 32 * a.KS1 + n0 / 16 + k) * 2) * 64 + lane;
-        d[0] = __builtin_bit_cast(uint4, f.p[0]);
-        d[64] = __builtin_bit_cast(uint4, f.p[1]);
+        u32x4_t *d = a.d1 + batch * a.b1 + ((m0 / 32 * a.KS1 + n0 / 16 + k) * 2) * 64 + lane;
+        d[0] = __builtin_bit_cast(u32x4_t, f.p[0]);
+        d[64] = __builtin_bit_cast(u32x4_t, f.p[1]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -356,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void ns_prod64(Prod a, Mat out, T *y) {
     const int64_t batch = blockIdx.y;
     int64_t tm, tn;
     tile_of<MODE>(blockIdx.x, a.tn, tm, tn);
-    const uint4 *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
+    const u32x4_t *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
     f32x16_t acc[2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -391,15 +400,15 @@ __global__ __launch_bounds__(kThreads) void ns_prod64(Prod a, Mat out, T *y) {
 // double-buffered LDS (one barrier each).
 template <int MODE, class T>
 __global__ __launch_bounds__(kThreads, 2) void ns_prod128(Prod a, Mat out, T *y) {
-    constexpr int ST = 4 * 2 * 2 * 64;  // uint4 a stage of one operand: 4 row blocks, 2 steps, 2 planes
-    __shared__ uint4 lds[2][2][ST];
+    constexpr int ST = 4 * 2 * 2 * 64;  // u32x4_t a stage of one operand: 4 row blocks, 2 steps, 2 planes
+    __shared__ u32x4_t lds[2][2][ST];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
     const int64_t batch = blockIdx.y;
     int64_t tm, tn;
     tile_of<MODE>(blockIdx.x, a.tn, tm, tn);
     // thread t stages 16 bytes of each row block: 256 threads are the block's 2 steps of 2 planes
-    const uint4 *p = a.p + batch * a.bp + tm * 4 * a.KS * 128 + t, *q = a.q + batch * a.bq + tn * 4 * a.KS * 128 + t;
-    uint4 sp[4], sq[4];
+    const u32x4_t *p = a.p + batch * a.bp + tm * 4 * a.KS * 128 + t, *q = a.q + batch * a.bq + tn * 4 * a.KS * 128 + t;
+    u32x4_t sp[4], sq[4];
     auto fetch = [&](int64_t k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -468,7 +477,7 @@ inline Plan plan_of(int64_t batch, int64_t S, int64_t L) {
     p.tile = n128 >= 128 ? 128 : 64;
     p.Sp = up_to(S, p.tile);
     p.Lp = up_to(L, p.tile);
-    p.xsz = p.Sp * p.Lp / 4;  // uint4: 4 bytes an element
+    p.xsz = p.Sp * p.Lp / 4;  // u32x4_t: 4 bytes an element
     p.asz = p.Sp * p.Sp / 4;
     p.bytes = batch * (3 * p.xsz + 2 * p.asz) * 16 + batch * kSumBlocks * 8;
     return p;
@@ -487,7 +496,7 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
         return launch_status(fn);
     }
     Work w{};
-    uint4 *c = static_cast<uint4 *>(ws);
+    u32x4_t *c = static_cast<u32x4_t *>(ws);
     w.x = c, c += batch * p.xsz;
     w.xt[0] = c, c += batch * p.xsz;
     w.xt[1] = c, c += batch * p.xsz;
@@ -508,7 +517,7 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
         else hipLaunchKernelGGL((ns_prod64<M, T>), dim3(n, nb), dim3(kThreads), 0, st, a, out, dst);
     };
     for (int32_t s = 0; s < steps; ++s) {
-        uint4 *cur = w.xt[s & 1], *nxt = w.xt[(s + 1) & 1];
+        u32x4_t *cur = w.xt[s & 1], *nxt = w.xt[(s + 1) & 1];
         go(std::integral_constant<int, kGram>(),
            Prod{w.x, w.x, w.bx, w.bx, kl, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f}, tri);
         go(std::integral_constant<int, kPoly>(),

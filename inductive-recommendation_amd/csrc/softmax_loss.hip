@@ -47,19 +47,19 @@ inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
 
 // A packed table: its blocks, then one exponent per block.
 struct Packed {
-    const uint4 *blocks;
+    const u32x4_t *blocks;
     const int32_t *exps;
 };
 inline Packed packed_view(const void *p, int64_t rows, int32_t dtype, int dp) {
     const char *c = static_cast<const char *>(p);
-    return Packed{reinterpret_cast<const uint4 *>(c),
+    return Packed{reinterpret_cast<const u32x4_t *>(c),
                   reinterpret_cast<const int32_t *>(c + blocks_of(rows) * block_bytes(dtype, dp))};
 }
 
 struct PackArgs {
     int64_t rows, ld;
     const void *src;
-    uint4 *blocks;
+    u32x4_t *blocks;
     int32_t *exps;
     const int64_t *target;  // rows whose target is `ignore` are packed as zeros; NULL: none
     int64_t ignore;
@@ -87,9 +87,9 @@ __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, 
         for (int i = t; i < kRB * DP / VE; i += kThreads) {
             const int r = i / (DP / VE), c = (i % (DP / VE)) * VE;
             const int64_t gr = r0 + r;
-            uint4 raw = make_uint4(0, 0, 0, 0);
+            u32x4_t raw = u32x4_t{0, 0, 0, 0};
             if (gr < a.rows && c < d && !(a.target && a.target[gr] == a.ignore))
-                raw = *reinterpret_cast<const uint4 *>(src + gr * a.ld + c);
+                raw = *reinterpret_cast<const u32x4_t *>(src + gr * a.ld + c);
             typename P::elem e[VE];
             __builtin_memcpy(e, &raw, 16);
 #pragma unroll
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, 
         s = pow2f(P::kOff - e);
     }
     if (t == 0) a.exps[blk] = e;
-    uint4 *out = a.blocks + blk * (block_halves<P>(DP) / 8);
+    u32x4_t *out = a.blocks + blk * (block_halves<P>(DP) / 8);
     constexpr int KS = DP / 16, DB = DP / 32;
     const int lane = t & 63, col = lane & 31, h = lane >> 5;
     for (int f = t >> 6; f < 2 * KS; f += kThreads / 64) {
@@ -133,13 +133,13 @@ __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, 
         Frags<P> fr;
         split8(v, fr);
 #pragma unroll
-        for (int n = 0; n < P::NS; ++n) out[(f * P::NS + n) * 64 + lane] = __builtin_bit_cast(uint4, fr.p[n]);
+        for (int n = 0; n < P::NS; ++n) out[(f * P::NS + n) * 64 + lane] = __builtin_bit_cast(u32x4_t, fr.p[n]);
     }
     static_assert(DB * 2 == KS, "T part has as many fragments as the S part");
 }
 
 template <class P>
-__device__ __forceinline__ void load_frags(const uint4 *base, int f, int lane, Frags<P> &fr) {
+__device__ __forceinline__ void load_frags(const u32x4_t *base, int f, int lane, Frags<P> &fr) {
 #pragma unroll
     for (int n = 0; n < P::NS; ++n)
         fr.p[n] = __builtin_bit_cast(typename P::frag, base[(f * P::NS + n) * 64 + lane]);
@@ -158,10 +158,9 @@ struct FwdArgs {
 template <class P, int DP, int NB, bool WITH_O>
 __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32;
-    constexpr int TILE = block_halves<P>(DP) / 8 / (WITH_O ? 1 : 2);  // uint4 of a streamed block
+    constexpr int TILE = block_halves<P>(DP) / 8 / (WITH_O ? 1 : 2);  // u32x4_t of a streamed block
     constexpr int BLK = block_halves<P>(DP) / 8;
-    constexpr int NST = (TILE + kThreads - 1) / kThreads;
-    __shared__ uint4 lds[2][TILE];
+    __shared__ u32x4_t lds0[TILE], lds1[TILE];
     __shared__ int32_t cmax_s;
     // workgroups of one split sit on one XCD (blockIdx % 8), next to each other in time: the
     // split's item blocks come from that XCD's L2 for all batch tiles but the first
@@ -190,7 +189,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
     float c_x[NB], m[NB], z[NB], tl[NB];
     int tgt[NB];
     bool live[NB];
-    f32x16_t o[NB][WITH_O ? DB : 1];
+    f32x16_t o[WITH_O ? DB : 1][NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         const int64_t xb = (bt * 4 + wave) * NB + n;
@@ -208,29 +207,19 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
 #pragma unroll
         for (int q = 0; q < (WITH_O ? DB : 1); ++q)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[n][q][i] = 0.f;
+            for (int i = 0; i < 16; ++i) o[q][n][i] = 0.f;
     }
 
-    uint4 st[NST];
-    auto fetch = [&](int64_t k) {
-        const uint4 *src = a.w.blocks + k * BLK;
-#pragma unroll
-        for (int i = 0; i < NST; ++i)
-            if (TILE % kThreads == 0 || i * kThreads + t < TILE) st[i] = src[i * kThreads + t];
-    };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NST; ++i)
-            if (TILE % kThreads == 0 || i * kThreads + t < TILE) lds[buf][i * kThreads + t] = st[i];
-    };
-    fetch(k0);
-    stage(0);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k = k0; k < k1; ++k, buf ^= 1) {
-        if (k + 1 < k1) fetch(k + 1);
-        const uint4 *w = lds[buf];
-        const int ew = P::kScaled ? __builtin_amdgcn_readfirstlane(a.w.exps[k]) : 0;
+    // w: the block in LDS that is used; next: the buffer that the following block is copied to meanwhile.
+    // (Two arrays by name, and the loop in pairs: so the compiler sees that reading one need not wait for
+    // the copy into the other.)
+    int ew_next = P::kScaled ? a.w.exps[k0] : 0;  // loaded a block ahead, before that block's copy is begun
+    auto step = [&](int64_t k, const u32x4_t *__restrict__ w, u32x4_t *__restrict__ next) {
+        const int ew = P::kScaled ? __builtin_amdgcn_readfirstlane(ew_next) : 0;
+        if (k + 1 < k1) {
+            if (P::kScaled) ew_next = a.w.exps[k + 1];
+            copy_to_lds<TILE>(a.w.blocks + (k + 1) * BLK, next, t);
+        }
         const float c_w = P::kScaled ? pow2f(ew - P::kOff) : 1.f;
         f32x16_t acc[NB];
 #pragma unroll
@@ -241,8 +230,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
         for (int s = 0; s < KS; ++s) {
             Frags<P> wf;
             load_frags<P>(w, s, lane, wf);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) acc[n] = mfma_split<P>(wf, xf[n][s], acc[n]);
+            mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return xf[n][s]; }, acc);
         }
         const int v0 = (int)(k * kRB);
         const int nv = a.V - k * kRB < kRB ? (int)(a.V - k * kRB) : kRB;  // items of this block
@@ -274,7 +262,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
 #pragma unroll
                     for (int q = 0; q < DB; ++q)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[n][q][i] *= f;
+                        for (int i = 0; i < 16; ++i) o[q][n][i] *= f;
                 }
             }
             // weights p 2^sh: up to 2^14 in the halves' range, less where the block's rows are
@@ -308,17 +296,22 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
         }
         if constexpr (WITH_O) {
 #pragma unroll
-            for (int q = 0; q < DB; ++q)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    Frags<P> wf;
-                    load_frags<P>(w, KS + 2 * q + s, lane, wf);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) o[n][q] = mfma_split<P>(wf, pf[n][s], o[n][q]);
-                }
+            for (int f = 0; f < 2 * DB; ++f) {
+                Frags<P> wf;
+                load_frags<P>(w, KS + f, lane, wf);
+                f32x16_t (&of)[NB] = o[f >> 1];
+                mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
+            }
         }
-        if (k + 1 < k1) stage(buf ^ 1);
+        copies_done();
         __syncthreads();
+    };
+    copy_to_lds<TILE>(a.w.blocks + k0 * BLK, lds0, t);
+    copies_done();
+    __syncthreads();
+    for (int64_t k = k0; k < k1; k += 2) {
+        step(k, lds0, lds1);
+        if (k + 1 < k1) step(k + 1, lds1, lds0);
     }
     if (WITH_O && bt == 0 && t == 0) a.pc[split] = C;
 #pragma unroll
@@ -341,7 +334,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
                     *reinterpret_cast<float4 *>(dst + q * 32 + g * 8 + h * 4) =
-                        make_float4(o[n][q][4 * g], o[n][q][4 * g + 1], o[n][q][4 * g + 2], o[n][q][4 * g + 3]);
+                        make_float4(o[q][n][4 * g], o[q][n][4 * g + 1], o[q][n][4 * g + 2], o[q][n][4 * g + 3]);
         }
     }
 }
@@ -560,7 +553,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
     constexpr int KS = DP / 16, DB = DP / 32;
     constexpr int BLK = block_halves<P>(DP) / 8;
     constexpr int NST = (BLK + kThreads - 1) / kThreads;
-    __shared__ uint4 lds[2][BLK];
+    __shared__ u32x4_t lds[2][BLK];
     __shared__ float info[2][3][kRB];  // off, hot, target of the streamed block
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
     const int64_t nvb = blocks_of(a.V), nxb = blocks_of(a.B);
@@ -571,7 +564,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
     float c_w[NB];
     int v0[NB];
     bool live[NB];
-    f32x16_t o[NB][DB];
+    f32x16_t o[DB][NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
         const int64_t vb = ((int64_t)blockIdx.x * 4 + wave) * NB + n;
@@ -584,13 +577,13 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
 #pragma unroll
         for (int q = 0; q < DB; ++q)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[n][q][i] = 0.f;
+            for (int i = 0; i < 16; ++i) o[q][n][i] = 0.f;
     }
 
-    uint4 st[NST];
+    u32x4_t st[NST];
     float si = 0.f;
     auto fetch = [&](int64_t k) {
-        const uint4 *src = a.x.blocks + k * BLK;
+        const u32x4_t *src = a.x.blocks + k * BLK;
 #pragma unroll
         for (int i = 0; i < NST; ++i)
             if (BLK % kThreads == 0 || i * kThreads + t < BLK) st[i] = src[i * kThreads + t];
@@ -610,7 +603,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
     int buf = 0;
     for (int64_t k = k0; k < k1; ++k, buf ^= 1) {
         if (k + 1 < k1) fetch(k + 1);
-        const uint4 *x = lds[buf];
+        const u32x4_t *x = lds[buf];
         const float c_x = P::kScaled ? pow2f(__builtin_amdgcn_readfirstlane(a.x.exps[k]) - P::kOff) : 1.f;
         const bool neg = __builtin_amdgcn_readfirstlane(a.info.neg[k]) != 0;
         f32x16_t acc[NB];
@@ -618,12 +611,12 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+        Frags<P> xf[2];
+        load_frags<P>(x, 0, lane, xf[0]);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            Frags<P> xf;
-            load_frags<P>(x, s, lane, xf);
-#pragma unroll
-            for (int n = 0; n < NB; ++n) acc[n] = mfma_split<P>(xf, wf[n][s], acc[n]);
+            load_frags<P>(x, s + 1, lane, xf[(s + 1) & 1]);
+            mfma_row<P, NB>(xf[s & 1], [&](int n) -> const Frags<P> & { return wf[n][s]; }, acc);
         }
         // lane: item v0 + col; register i: batch row 8 (i/4) + 4 h + i%4 of the block
         float off[16];
@@ -660,14 +653,11 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
             split8(ph, pf[n][1]);
         }
 #pragma unroll
-        for (int q = 0; q < DB; ++q)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                Frags<P> xf;
-                load_frags<P>(x, KS + 2 * q + s, lane, xf);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) o[n][q] = mfma_split<P>(xf, pf[n][s], o[n][q]);
-            }
+        for (int f = 0; f < 2 * DB; ++f) {
+            if (f + 1 < 2 * DB) load_frags<P>(x, KS + f + 1, lane, xf[(KS + f + 1) & 1]);
+            f32x16_t (&of)[NB] = o[f >> 1];
+            mfma_row<P, NB>(xf[(KS + f) & 1], [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
+        }
         if (k + 1 < k1) stage(buf ^ 1);
         __syncthreads();
     }
@@ -681,8 +671,8 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int c = q * 32 + g * 8 + h * 4;
-                const float w0 = o[n][q][4 * g] * f, w1 = o[n][q][4 * g + 1] * f, w2 = o[n][q][4 * g + 2] * f,
-                            w3 = o[n][q][4 * g + 3] * f;
+                const float w0 = o[q][n][4 * g] * f, w1 = o[q][n][4 * g + 1] * f, w2 = o[q][n][4 * g + 2] * f,
+                            w3 = o[q][n][4 * g + 3] * f;
                 if (a.splits > 1)
                     *reinterpret_cast<float4 *>(a.part + (split * a.V + v) * DP + c) = make_float4(w0, w1, w2, w3);
                 else
@@ -838,9 +828,9 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
             const int64_t nx = blocks_of(b), nw = blocks_of(v), eb = dtype_bytes(dtype);
             const bool vec = d * eb % 16 == 0 && ldx * eb % 16 == 0 && ld_items * eb % 16 == 0 && aligned16(x) &&
                              aligned16(items);
-            PackArgs px{b, ldx, x, const_cast<uint4 *>(a.x.blocks), const_cast<int32_t *>(a.x.exps), target,
+            PackArgs px{b, ldx, x, const_cast<u32x4_t *>(a.x.blocks), const_cast<int32_t *>(a.x.exps), target,
                         ignore_index};
-            PackArgs pw{v, ld_items, items, const_cast<uint4 *>(a.w.blocks), const_cast<int32_t *>(a.w.exps), nullptr, 0};
+            PackArgs pw{v, ld_items, items, const_cast<u32x4_t *>(a.w.blocks), const_cast<int32_t *>(a.w.exps), nullptr, 0};
             const FwdPlan plan = fwd_plan(b, v, dp);
             const int64_t grid = (a.splits + 7) / 8 * 8 * a.nbt;
             if (grid > INT32_MAX || nx + nw > INT32_MAX) return arg_error(fn, "too many workgroups");

@@ -106,4 +106,4 @@ def test_newton_schulz_c_arguments():
         assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
     assert ns(batch=0) == 0 and ns(rows=0) == 0
     assert lib.igr_newton_schulz_workspace_size(6, 64, 64) == 0  # one workgroup a matrix
-    assert lib.igr_newton_schulz_workspace_size(1, 128, 512) == (3 * 128 * 512 + 2 * 128 * 128) * 4 + 64 * 8
+    assert lib.igr_newton_schulz_workspace_size(1, 128, 512) == (3 * 128 * 512 + 2 * 128 * 128) * 4 + 256 * 8
