@@ -135,50 +135,43 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
             }
         }
     };
+    // K steps of two fragment rows; the three parts of the product in sums of their own, so that
+    // the MFMAs, 3 K in a row otherwise, wait for each other a third as long
+    auto product = [&](const u32x4_t *p, int p0, const u32x4_t *q, int q0, auto ks) {
+        constexpr int K = decltype(ks)::value;
+        f32x16_t c0, c1, c2;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c0[i] = c1[i] = c2[i] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            Frag2 fp, fq;
+            load2(p, p0 + k, lane, fp);
+            load2(q, q0 + k, lane, fq);
+            c0 = mfma32(fp.p[0], fq.p[1], c0);
+            c1 = mfma32(fp.p[1], fq.p[0], c1);
+            c2 = mfma32(fp.p[0], fq.p[0], c2);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c2[i] += c0[i] + c1[i];
+        return c2;
+    };
     store_x();
     __syncthreads();
     for (int s = 0; s < steps; ++s) {
-        f32x16_t acc;
         float av[16], v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < KL; ++k) {
-            Frag2 p, q;
-            load2(xs, nb0 * KL + k, lane, p);
-            load2(xs, mb * KL + k, lane, q);
-            acc = mfma_split<SplitF32>(p, q, acc);
-        }
+        f32x16_t acc = product(xs, nb0 * KL, xs, mb * KL, std::integral_constant<int, KL>());
 #pragma unroll
         for (int i = 0; i < 16; ++i) av[i] = acc[i] * down;
         put_block(am, mb, 4, nb0 * 32, av, lane);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            Frag2 p, q;
-            load2(am, nb0 * 4 + k, lane, p);
-            load2(am, mb * 4 + k, lane, q);
-            acc = mfma_split<SplitF32>(p, q, acc);
-        }
+        acc = product(am, nb0 * 4, am, mb * 4, std::integral_constant<int, 4>());
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = fmaf(cb, av[i], cc * (acc[i] * down));
         put_block(qm, mb, 4, nb0 * 32, v, lane);
         __syncthreads();
-        Frag2 qf[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) load2(qm, mb * 4 + k, lane, qf[k]);
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                Frag2 q;
-                load2(xt, (nb0 + 2 * j) * 4 + k, lane, q);
-                acc = mfma_split<SplitF32>(qf[k], q, acc);
-            }
+            acc = product(qm, mb * 4, xt, (nb0 + 2 * j) * 4, std::integral_constant<int, 4>());
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[j][i] = fmaf(ca, x[j][i], acc[i] * down);
         }
@@ -290,7 +283,7 @@ struct Prod {
     const u32x4_t *p, *q;     // fragment matrices: rows of the result, columns of the result
     int64_t bp, bq;         // batch strides
     int64_t KS;             // 16-column steps of both
-    int64_t tn;             // tiles along the columns (kUpdate, kLast)
+    int64_t tiles, tm;      // tiles, and those along the rows (kUpdate, kLast)
     u32x4_t *d0, *d1;         // result as rows = its columns (straight) and rows = its rows (turned)
     int64_t KS0, KS1, b0, b1;
     const u32x4_t *add;       // what is added, with d0's layout
@@ -343,119 +336,147 @@ __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_
     __builtin_amdgcn_wave_barrier();
 }
 
+// The tile of a workgroup: each XCD (blockIdx % 8) takes a run of consecutive tiles, so that tiles which
+// share operand rows share an L2.  False for the surplus workgroups of the last run.
 template <int MODE>
-__device__ __forceinline__ void tile_of(int64_t id, int64_t tn, int64_t &m, int64_t &n) {
+__device__ __forceinline__ bool tile_of(const Prod &a, int64_t &m, int64_t &n) {
+    const int64_t id = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (id >= a.tiles) return false;
     if constexpr (MODE == kGram || MODE == kPoly) {  // tiles on and below the diagonal, row by row
         m = (int64_t)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
         while (m * (m + 1) / 2 > id) --m;
         while ((m + 1) * (m + 2) / 2 <= id) ++m;
         n = id - m * (m + 1) / 2;
-    } else {
-        m = id / tn;
-        n = id % tn;
+    } else {  // column by column
+        m = id % a.tm;
+        n = id / a.tm;
     }
+    return true;
 }
 
-// Few tiles: 64 x 64 a workgroup, the contraction dealt out to its four waves, which load fragments straight
-// from memory and join their sums in LDS in wave order.
-template <int MODE, class T>
-__global__ __launch_bounds__(kThreads) void ns_prod64(Prod a, Mat out, T *y) {
-    __shared__ float part[4][4][16][64];
+// Few tiles: BT x BT blocks a workgroup, the contraction dealt out to its NW waves, which load fragments
+// straight from memory (four steps in flight) and join their sums in LDS in wave order.
+template <int MODE, class T, int BT, int NW>
+__global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) {
+    __shared__ float part[NW][BT * BT][16][64];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int64_t batch = blockIdx.y;
     int64_t tm, tn;
-    tile_of<MODE>(blockIdx.x, a.tn, tm, tn);
+    if (!tile_of<MODE>(a, tm, tn)) return;
     const u32x4_t *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
-    f32x16_t acc[2][2];
+    f32x16_t acc[BT][BT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < BT * BT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i >> 1][i & 1][r] = 0.f;
-    for (int64_t k = wave; k < a.KS; k += 4) {
-        Frag2 fp[2], fq[2];
+        for (int r = 0; r < 16; ++r) acc[i / BT][i % BT][r] = 0.f;
+    auto multiply = [&](int64_t k, auto steps) {
+        constexpr int N = decltype(steps)::value;
+        Frag2 fp[N][BT], fq[N][BT];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            load2(p, (tm * 2 + i) * a.KS + k, lane, fp[i]);
-            load2(q, (tn * 2 + i) * a.KS + k, lane, fq[i]);
-        }
+        for (int s = 0; s < N; ++s)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = mfma_split<SplitF32>(fp[i >> 1], fq[i & 1], acc[i >> 1][i & 1]);
-    }
+            for (int i = 0; i < BT; ++i) {
+                load2(p, (tm * BT + i) * a.KS + k + s * NW, lane, fp[s][i]);
+                load2(q, (tn * BT + i) * a.KS + k + s * NW, lane, fq[s][i]);
+            }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int s = 0; s < N; ++s)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) part[wave][i][r][lane] = acc[i >> 1][i & 1][r];
+            for (int i = 0; i < BT; ++i)
+                mfma_row<SplitF32, BT>(fp[s][i], [&](int n) -> const Frag2 & { return fq[s][n]; }, acc[i]);
+    };
+    int64_t k = wave;
+    for (; k + 3 * NW < a.KS; k += 4 * NW) multiply(k, std::integral_constant<int, 4>());
+    for (; k < a.KS; k += NW) multiply(k, std::integral_constant<int, 1>());
+#pragma unroll
+    for (int i = 0; i < BT * BT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[wave][i][r][lane] = acc[i / BT][i % BT][r];
     __syncthreads();
     f32x16_t s;
+    if (wave < BT * BT) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-        s[r] = (part[0][wave][r][lane] + part[1][wave][r][lane]) + (part[2][wave][r][lane] + part[3][wave][r][lane]);
+        for (int r = 0; r < 16; ++r) {
+            s[r] = part[0][wave][r][lane];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) s[r] += part[w][wave][r][lane];
+        }
+    }
     __syncthreads();
+    if (wave >= BT * BT) return;
     const bool mirror = MODE == kUpdate || tm != tn;
-    emit<MODE, T>(a, out, y, batch, (tm * 2 + (wave >> 1)) * 32, (tn * 2 + (wave & 1)) * 32, mirror, s,
-                  reinterpret_cast<float (*)[33]>(&part[wave][0][0][0]), lane);
+    emit<MODE, T>(a, out, y, batch, (tm * BT + wave / BT) * 32, (tn * BT + wave % BT) * 32, mirror, s,
+                  reinterpret_cast<float (*)[33]>(&part[wave * (BT == 1 ? 2 : 1)][0][0][0]), lane);
 }
 
-// Many tiles: 128 x 128 a workgroup, four waves of 64 x 64, two 16-column steps at a time through
-// double-buffered LDS (one barrier each).
+// Many tiles: 128 x 128 a workgroup, four waves of 64 x 64, two 16-column steps at a time.  The rows'
+// operand goes through double-buffered LDS (one barrier each), the columns' straight to registers, a
+// stage ahead: with both in LDS its reads and writes, 128 bytes a clock and CU at the full MFMA rate, were
+// all that LDS gives; like this LDS gives 64 and the vector cache 43.
 template <int MODE, class T>
 __global__ __launch_bounds__(kThreads, 2) void ns_prod128(Prod a, Mat out, T *y) {
-    constexpr int ST = 4 * 2 * 2 * 64;  // u32x4_t a stage of one operand: 4 row blocks, 2 steps, 2 planes
-    __shared__ u32x4_t lds[2][2][ST];
+    constexpr int ST = 4 * 2 * 2 * 64;  // 16-byte groups of a stage: 4 row blocks, 2 steps, 2 planes
+    __shared__ u32x4_t lds[2][ST];
+    __shared__ float turn[4][32][33];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
     const int64_t batch = blockIdx.y;
     int64_t tm, tn;
-    tile_of<MODE>(blockIdx.x, a.tn, tm, tn);
+    if (!tile_of<MODE>(a, tm, tn)) return;
     // thread t stages 16 bytes of each row block: 256 threads are the block's 2 steps of 2 planes
-    const u32x4_t *p = a.p + batch * a.bp + tm * 4 * a.KS * 128 + t, *q = a.q + batch * a.bq + tn * 4 * a.KS * 128 + t;
-    u32x4_t sp[4], sq[4];
+    const u32x4_t *p = a.p + batch * a.bp + tm * 4 * a.KS * 128 + t;
+    const u32x4_t *q = a.q + batch * a.bq;
+    u32x4_t sp[4];
     auto fetch = [&](int64_t k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            sp[i] = p[(i * a.KS + k) * 128];
-            sq[i] = q[(i * a.KS + k) * 128];
-        }
+        for (int i = 0; i < 4; ++i) sp[i] = p[(i * a.KS + k) * 128];
     };
     auto stage = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            lds[buf][0][i * 256 + t] = sp[i];
-            lds[buf][1][i * 256 + t] = sq[i];
-        }
+        for (int i = 0; i < 4; ++i) lds[buf][i * 256 + t] = sp[i];
+    };
+    auto columns = [&](int64_t k, Frag2 (&f)[2][2]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) load2(q, (tn * 4 + wn * 2 + i) * a.KS + k + s, lane, f[s][i]);
     };
     f32x16_t acc[2][2];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i >> 1][i & 1][r] = 0.f;
+    Frag2 f0[2][2], f1[2][2];
     fetch(0);
+    columns(0, f0);
     stage(0);
     __syncthreads();
-    int buf = 0;
-    for (int64_t k = 0; k < a.KS; k += 2, buf ^= 1) {
+    auto step = [&](int64_t k, int buf, Frag2 (&now)[2][2], Frag2 (&next)[2][2]) {
         const bool more = k + 2 < a.KS;
-        if (more) fetch(k + 2);
+        if (more) {
+            fetch(k + 2);
+            columns(k + 2, next);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            Frag2 fp[2], fq[2];
+            Frag2 fp[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                load2(lds[buf][0], (wm * 2 + i) * 2 + s, lane, fp[i]);
-                load2(lds[buf][1], (wn * 2 + i) * 2 + s, lane, fq[i]);
-            }
+            for (int i = 0; i < 2; ++i) load2(lds[buf], (wm * 2 + i) * 2 + s, lane, fp[i]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[i >> 1][i & 1] = mfma_split<SplitF32>(fp[i >> 1], fq[i & 1], acc[i >> 1][i & 1]);
+            for (int i = 0; i < 2; ++i)
+                mfma_row<SplitF32, 2>(fp[i], [&](int n) -> const Frag2 & { return now[s][n]; }, acc[i]);
         }
         if (more) stage(buf ^ 1);
         __syncthreads();
+    };
+    for (int64_t k = 0; k < a.KS; k += 4) {  // KS is a multiple of 8
+        step(k, 0, f0, f1);
+        step(k + 2, 1, f1, f0);
     }
     const bool mirror = MODE == kUpdate || tm != tn;
-    float(*turn)[33] = reinterpret_cast<float(*)[33]>(reinterpret_cast<float *>(&lds[0][0][0]) + wave * 32 * 33);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         emit<MODE, T>(a, out, y, batch, (tm * 4 + wm * 2 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32, mirror,
-                      acc[i >> 1][i & 1], turn, lane);
+                      acc[i >> 1][i & 1], turn[wave], lane);
 }
 
 // ------------------------------------------------------------------ host side
@@ -472,9 +493,9 @@ inline Plan plan_of(int64_t batch, int64_t S, int64_t L) {
     Plan p{};
     p.small = S <= 64 && L <= 256;
     if (p.small) return p;
-    // 128-wide tiles once the update has enough of them for half the chip
-    const int64_t n128 = ((S + 127) / 128) * ((L + 127) / 128) * batch;
-    p.tile = n128 >= 128 ? 128 : 64;
+    // 128-wide tiles once the update has enough of them for half the chip, 64-wide ones for a quarter
+    auto tiles = [&](int64_t t) { return ((S + t - 1) / t) * ((L + t - 1) / t) * batch; };
+    p.tile = tiles(128) >= 128 ? 128 : tiles(64) >= 256 ? 64 : 32;
     p.Sp = up_to(S, p.tile);
     p.Lp = up_to(L, p.tile);
     p.xsz = p.Sp * p.Lp / 4;  // u32x4_t: 4 bytes an element
@@ -509,35 +530,53 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
     const int64_t blocks = (p.Sp / 32) * (p.Lp / 32);
     hipLaunchKernelGGL((ns_pack<T>), dim3((unsigned)((blocks + 3) / 4), nb), dim3(kThreads), 0, st, in, src, part, eps, w);
     const int64_t ts = p.Sp / p.tile, tl = p.Lp / p.tile;
-    const unsigned tri = (unsigned)(ts * (ts + 1) / 2), all = (unsigned)(ts * tl);
+    const int64_t tri = ts * (ts + 1) / 2, all = ts * tl;
     const int64_t ks = p.Sp / 16, kl = p.Lp / 16;
-    auto go = [&](auto mode, const Prod &a, unsigned n) {
+    auto go = [&](auto mode, const Prod &a) {
+        const unsigned n = (unsigned)((a.tiles + 7) / 8 * 8);
         constexpr int M = decltype(mode)::value;
         if (p.tile == 128) hipLaunchKernelGGL((ns_prod128<M, T>), dim3(n, nb), dim3(kThreads), 0, st, a, out, dst);
-        else hipLaunchKernelGGL((ns_prod64<M, T>), dim3(n, nb), dim3(kThreads), 0, st, a, out, dst);
+        else if (p.tile == 64) hipLaunchKernelGGL((ns_prod_split<M, T, 2, 4>), dim3(n, nb), dim3(256), 0, st, a, out, dst);
+        else hipLaunchKernelGGL((ns_prod_split<M, T, 1, 8>), dim3(n, nb), dim3(512), 0, st, a, out, dst);
     };
     for (int32_t s = 0; s < steps; ++s) {
         u32x4_t *cur = w.xt[s & 1], *nxt = w.xt[(s + 1) & 1];
         go(std::integral_constant<int, kGram>(),
-           Prod{w.x, w.x, w.bx, w.bx, kl, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f}, tri);
+           Prod{w.x, w.x, w.bx, w.bx, kl, tri, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f});
         go(std::integral_constant<int, kPoly>(),
-           Prod{w.a, w.a, w.ba, w.ba, ks, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc}, tri);
-        const Prod u{w.q, cur, w.ba, w.bx, ks, tl, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f};
-        if (s + 1 < steps) go(std::integral_constant<int, kUpdate>(), u, all);
-        else go(std::integral_constant<int, kLast>(), u, all);
+           Prod{w.a, w.a, w.ba, w.ba, ks, tri, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc});
+        const Prod u{w.q, cur, w.ba, w.bx, ks, all, ts, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f};
+        if (s + 1 < steps) go(std::integral_constant<int, kUpdate>(), u);
+        else go(std::integral_constant<int, kLast>(), u);
     }
     return launch_status(fn);
 }
 
-// The iterates of every singular value in [0, 1]: the fixed scale holds X up to 4 and Q up to 16.
+// The fixed scale holds X up to 4 and Q up to 16: follow the interval [0, hi] of singular values through the
+// steps, each image's bound from the ends and the critical points of the odd quintic.
 inline bool coefficients_fit(int32_t steps, double a, double b, double c) {
-    for (int i = 0; i <= 2000; ++i) {
-        double x = (double)i / 2000;
-        for (int32_t s = 0; s < steps; ++s) {
-            const double l = x * x, q = b * l + c * l * l;
-            x = a * x + q * x;
-            if (!(std::fabs(x) <= 4.) || !(std::fabs(q) <= 16.)) return false;
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+    double hi = 1.;
+    for (int32_t s = 0; s < steps; ++s) {
+        double x = 0., q = 0.;
+        auto at = [&](double l) {  // l = sigma^2
+            if (l < 0. || l > hi * hi) return;
+            q = std::max(q, std::fabs(b * l + c * l * l));
+            x = std::max(x, std::sqrt(l) * std::fabs(a + b * l + c * l * l));
+        };
+        at(hi * hi);
+        if (c != 0.) {
+            at(-b / (2. * c));  // of b l + c l^2
+            const double d = 9. * b * b - 20. * a * c;  // a + 3 b l + 5 c l^2 = 0
+            if (d >= 0.) {
+                at((-3. * b + std::sqrt(d)) / (10. * c));
+                at((-3. * b - std::sqrt(d)) / (10. * c));
+            }
+        } else if (b != 0.) {
+            at(-a / (3. * b));
         }
+        if (!(x <= 4.) || !(q <= 16.)) return false;
+        hi = x * (1. + 1e-5);  // roundings
     }
     return true;
 }

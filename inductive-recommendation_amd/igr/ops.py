@@ -12,6 +12,7 @@ DGL-compatible surface (the reference's operator API):
     gspmm(g, 'copy_rhs', 'sum'|'max', None, e) ~ dgl.ops.gspmm   model.py:4270, 4273
     gsddmm(g, 'dot', lhs, rhs)                 ~ AttIGCN.masked_mm model.py:4246-4255
 """
+import contextlib
 import ctypes
 import weakref
 import math
@@ -1221,6 +1222,14 @@ def _same_device(*ts):
         raise IgrError(f'tensors on different devices: {sorted(map(str, dev))}')
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """The device's context, so that buffers and the stream are its own; nothing to switch if it is current."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _buffer(nbytes, device):
     return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
 
@@ -1239,7 +1248,7 @@ class SoftmaxLoss(torch.autograd.Function):
         (B, d), V, dev = xs.shape, ws.shape[0], xs.device
         need_x, need_w = ctx.needs_input_grad[:2]
         lib = L.lib()
-        with torch.cuda.device(dev):
+        with _on(dev):
             packs = [_buffer(lib.igr_softmax_loss_pack_size(n, d, dt), dev) for n in (B, V)]
             loss, lse = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
             total = count = o = None
@@ -1264,7 +1273,7 @@ class SoftmaxLoss(torch.autograd.Function):
         dt, B, V, d, scale, ignore_index, reduction = ctx.args
         ws, ldw, _ = _table(items, 'softmax_loss items')
         dev = ws.device
-        with torch.cuda.device(dev):
+        with _on(dev):
             grad = _f32(grad).contiguous()
             dx = torch.empty(B, d, dtype=ws.dtype, device=dev) if ctx.needs_input_grad[0] else None
             dw = None
@@ -1317,7 +1326,7 @@ def quantize_rows(x):
     xs, ldx, dt = _table(x.detach(), 'quantize_rows')
     n, k = xs.shape
     ldq = (k + 15) // 16 * 16
-    with torch.cuda.device(xs.device):
+    with _on(xs.device):
         q = torch.empty(n, ldq, dtype=torch.int8, device=xs.device)
         scale = torch.empty(n, dtype=torch.float32, device=xs.device)
         L.call('igr_quantize_rows', dt, n, k, _p(xs), ldx, _p(q), ldq, _p(scale), _stream())
@@ -1348,7 +1357,7 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):
         return t, max(t.stride(0), k)
     a, lda = rows(a)
     b, ldb = rows(b)
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         c = torch.empty(m, n, dtype=out_dtype, device=a.device)
         L.call('igr_gemm_int8', m, n, k, _p(a), lda, _p(a_scale.contiguous()), _p(b), ldb, _p(b_scale.contiguous()),
                _DTYPES[out_dtype], _p(c), n, _stream())
@@ -1374,7 +1383,7 @@ def newton_schulz(g, steps=5, coeffs=NEWTON_SCHULZ_COEFFS, eps=1e-7):
     b, r, c = x.shape
     if (x.stride(2) != 1 and c > 1) or x.stride(1) < c or x.stride(0) < 0:
         x = x.contiguous()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         out = torch.empty(b, r, c, dtype=x.dtype, device=x.device)
         wsb = L.lib().igr_newton_schulz_workspace_size(b, r, c)
         ws = _buffer(wsb, x.device) if wsb else None
