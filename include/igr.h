@@ -599,6 +599,25 @@ int igr_newton_schulz(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, 
                       int64_t stride_g, int32_t steps, double a, double b, double c, double eps, void *out,
                       void *workspace, int64_t ws_bytes, void *stream);
 
+/* What an orthogonalised step does around the products, for up to IGR_MUON_MAX_SLOTS fp32 weights in
+ * one launch (any alignment, contiguous, n elements each):
+ *   direction:  momentum <- mu momentum + grad,  direction = grad + mu momentum  (nesterov) or
+ *               momentum
+ *   apply:      param <- (1 - lr weight_decay) param - lr scale direction
+ * direction is then orthogonalised by igr_newton_schulz between the two (grad and momentum are
+ * not read by apply). */
+#define IGR_MUON_MAX_SLOTS 16
+typedef struct igr_muon_slot {
+    float *param;
+    const float *grad;
+    float *momentum;
+    float *direction;
+    int64_t n;
+} igr_muon_slot;
+int igr_muon_direction_f32(int32_t n_slots, const igr_muon_slot *slots, double mu, int32_t nesterov, void *stream);
+int igr_muon_apply_f32(int32_t n_slots, const igr_muon_slot *slots, double lr, double weight_decay, double scale,
+                       void *stream);
+
 #ifdef __cplusplus
 }
 #endif

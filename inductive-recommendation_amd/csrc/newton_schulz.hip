@@ -581,10 +581,78 @@ inline bool coefficients_fit(int32_t steps, double a, double b, double c) {
     return true;
 }
 
+// ------------------------------------------------------------------ around the products
+
+constexpr int kSlotBlocks = 64;  // workgroups a slot, striding over it
+
+struct Slots {
+    igr_muon_slot s[IGR_MUON_MAX_SLOTS];
+};
+
+// Elementwise and bound by memory: a launch reads and writes each weight's arrays once.
+__global__ __launch_bounds__(kThreads) void muon_direction(Slots a, float mu, int32_t nesterov) {
+    const igr_muon_slot s = a.s[blockIdx.y];
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < s.n; i += (int64_t)gridDim.x * kThreads) {
+        const float g = s.grad[i], m = fmaf(mu, s.momentum[i], g);
+        s.momentum[i] = m;
+        s.direction[i] = nesterov ? fmaf(mu, m, g) : m;
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void muon_apply(Slots a, float keep, float step) {
+    const igr_muon_slot s = a.s[blockIdx.y];
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < s.n; i += (int64_t)gridDim.x * kThreads)
+        s.param[i] = fmaf(-step, s.direction[i], keep * s.param[i]);
+}
+
+inline int take_slots(const char *fn, int32_t n_slots, const igr_muon_slot *slots, bool direction, Slots &a,
+                      unsigned &blocks) {
+    if (n_slots < 0 || n_slots > IGR_MUON_MAX_SLOTS) return arg_error(fn, "0 <= n_slots <= IGR_MUON_MAX_SLOTS");
+    if (n_slots > 0 && !slots) return arg_error(fn, "NULL slots");
+    int64_t most = 1;
+    for (int k = 0; k < n_slots; ++k) {
+        const igr_muon_slot &s = slots[k];
+        if (s.n <= 0) return arg_error(fn, "slot size must be positive");
+        if (!s.direction || (direction ? !s.grad || !s.momentum : !s.param)) return arg_error(fn, "NULL pointer in a slot");
+        a.s[k] = s;
+        most = std::max(most, (s.n + kThreads - 1) / kThreads);
+    }
+    blocks = (unsigned)std::min<int64_t>(most, n_slots > 4 ? kSlotBlocks : 4 * kSlotBlocks);
+    return IGR_OK;
+}
+
 }  // namespace
 }  // namespace igr
 
 using namespace igr;
+
+extern "C" int igr_muon_direction_f32(int32_t n_slots, const igr_muon_slot *slots, double mu, int32_t nesterov,
+                                      void *stream) {
+    return guarded("igr_muon_direction_f32", [&]() -> int {
+        const char *fn = "igr_muon_direction_f32";
+        Slots a;
+        unsigned blocks = 0;
+        if (int rc = take_slots(fn, n_slots, slots, true, a, blocks)) return rc;
+        if (n_slots == 0) return IGR_OK;
+        hipLaunchKernelGGL(muon_direction, dim3(blocks, (unsigned)n_slots), dim3(kThreads), 0,
+                           reinterpret_cast<hipStream_t>(stream), a, (float)mu, nesterov);
+        return launch_status(fn);
+    });
+}
+
+extern "C" int igr_muon_apply_f32(int32_t n_slots, const igr_muon_slot *slots, double lr, double weight_decay,
+                                  double scale, void *stream) {
+    return guarded("igr_muon_apply_f32", [&]() -> int {
+        const char *fn = "igr_muon_apply_f32";
+        Slots a;
+        unsigned blocks = 0;
+        if (int rc = take_slots(fn, n_slots, slots, false, a, blocks)) return rc;
+        if (n_slots == 0) return IGR_OK;
+        hipLaunchKernelGGL(muon_apply, dim3(blocks, (unsigned)n_slots), dim3(kThreads), 0,
+                           reinterpret_cast<hipStream_t>(stream), a, (float)(1. - lr * weight_decay), (float)(lr * scale));
+        return launch_status(fn);
+    });
+}
 
 extern "C" int64_t igr_newton_schulz_workspace_size(int64_t batch, int64_t rows, int64_t cols) {
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;

@@ -37,6 +37,13 @@ class IgrAdamSlot(ctypes.Structure):          # struct igr_adam_slot
     _fields_ = [('param', c_vp), ('grad', c_vp), ('exp_avg', c_vp), ('exp_avg_sq', c_vp), ('n', c_i64), ('step', c_i64)]
 
 
+MUON_MAX_SLOTS = 16
+
+
+class IgrMuonSlot(ctypes.Structure):          # struct igr_muon_slot
+    _fields_ = [('param', c_vp), ('grad', c_vp), ('momentum', c_vp), ('direction', c_vp), ('n', c_i64)]
+
+
 class IgrEpilogue(ctypes.Structure):
     """struct igr_epilogue (include/igr.h)."""
     _fields_ = [
@@ -138,6 +145,8 @@ SIGNATURES = {
     'igr_newton_schulz_workspace_size': (c_i64, [c_i64, c_i64, c_i64]),
     'igr_newton_schulz': (ctypes.c_int, [c_i32, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i32, ctypes.c_double,
                                          ctypes.c_double, ctypes.c_double, ctypes.c_double, c_vp, c_vp, c_i64, c_vp]),
+    'igr_muon_direction_f32': (ctypes.c_int, [c_i32, c_vp, ctypes.c_double, c_i32, c_vp]),
+    'igr_muon_apply_f32': (ctypes.c_int, [c_i32, c_vp, ctypes.c_double, ctypes.c_double, ctypes.c_double, c_vp]),
     'igr_loss_combine_f32': (ctypes.c_int, [c_vp, c_vp, c_vp, c_f32, c_f32, c_f32, c_vp, c_vp, c_vp]),
 }
 

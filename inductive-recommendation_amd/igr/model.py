@@ -154,6 +154,28 @@ class BasicModel(nn.Module):
             for t in tensors:
                 t.record_stream(cur)
 
+    def softmax_loss(self, users, pos_items, scale=1.0, need_l2=True):
+        """The full-catalogue form of bpr_loss: (mean softmax cross entropy of each user's positive item
+        against every item, mean l2 of the rows bpr_loss regularises, without negatives; None
+        when need_l2 is False).  scale = 1 / temperature."""
+        rep = self.get_rep()
+        self._join_batch_stream(users, pos_items)
+        loss = ops.softmax_loss(ops.gather(rep, users), rep[self.n_users:], pos_items, scale=scale)
+        if not need_l2:
+            return loss, None
+        t = self._l2_table(rep)
+        u, p = ops.gather(t, users), ops.gather(t, pos_items, self.n_users)
+        l2 = ops.Mean.apply((u ** 2).sum(1) + (p ** 2).sum(1))
+        extra = self._l2_extra()
+        return loss, (l2 if extra is None else l2 + extra)
+
+    def _l2_table(self, rep):
+        """The table whose batch rows the l2 term reads: rep, as in bpr_loss of most models."""
+        return rep
+
+    def _l2_extra(self):
+        return None
+
     def save(self, path):
         torch.save(self.state_dict(), path)
 
@@ -223,6 +245,9 @@ class LightGCN(BasicModel):
             return bpr, None
         _, l2 = ops.bpr_loss(self.embedding.weight, users, pos_items, neg_items, 0, self.n_users, keys=keys)
         return bpr, l2
+
+    def _l2_table(self, rep):
+        return self.embedding.weight
 
 
 class NGCF(BasicModel):

@@ -1178,6 +1178,20 @@ def means(a, b=None):
     return out
 
 
+class Mean(torch.autograd.Function):
+    """mean(x) of per-sample terms through igr_means_f32: fixed order, and one kernel whatever the length
+    (torch's own mean over many blocks clears a counter with a memset, which a captured step must not)."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.n = x.numel()
+        return means(x)[0]
+
+    @staticmethod
+    def backward(ctx, g):
+        return (g / ctx.n).expand(ctx.n)
+
+
 def loss_combine(bpr, l2=None, aux=None, c_l2=0.0, c_aux=0.0, loss_sum=None, weight=1.0):
     """loss = bpr + (c_l2 * l2 + c_aux * aux) as one launch on detached device
     scalars (trainer.py:551-552); loss_sum += loss * weight when given."""
@@ -1215,11 +1229,11 @@ def _table(t, what):
     return t, max(t.stride(0), t.shape[1]), _DTYPES[t.dtype]
 
 
-def _same_device(*ts):
-    _dev(*ts)
-    dev = {t.device for t in ts if t is not None}
-    if len(dev) > 1:
-        raise IgrError(f'tensors on different devices: {sorted(map(str, dev))}')
+def _same_device(first, *ts):
+    _dev(first, *ts)
+    for t in ts:
+        if t.device != first.device:
+            raise IgrError(f'tensors on different devices: {first.device}, {t.device}')
 
 
 _HERE = contextlib.nullcontext()
@@ -1227,7 +1241,12 @@ _HERE = contextlib.nullcontext()
 
 def _on(device):
     """The device's context, so that buffers and the stream are its own; nothing to switch if it is current."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _stream_of(device):
+    """The device's current stream, as _stream() without building a Stream object (3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _buffer(nbytes, device):
@@ -1260,7 +1279,7 @@ class SoftmaxLoss(torch.autograd.Function):
             wsb = lib.igr_softmax_loss_workspace_size(B, V, d, 0, int(need_x))
             L.call('igr_softmax_loss_fwd', dt, B, V, d, _p(xs), ldx, _p(ws), ldw, _p(target), ignore_index, scale,
                    int(reduction == 'mean'), _p(packs[0]), _p(packs[1]), _p(loss), _p(lse), _p(total), _p(count),
-                   _p(o), _p(_buffer(wsb, dev)), wsb, _stream())
+                   _p(o), _p(_buffer(wsb, dev)), wsb, _stream_of(dev))
         if need_x or need_w:
             ctx.save_for_backward(items, target, packs[0], packs[1], lse, count, o)
             ctx.args = (dt, B, V, d, scale, ignore_index, reduction)
@@ -1282,7 +1301,7 @@ class SoftmaxLoss(torch.autograd.Function):
             wsb = L.lib().igr_softmax_loss_workspace_size(B, V, d, 1, 0)
             L.call('igr_softmax_loss_bwd', dt, B, V, d, _p(ws), ldw, _p(target), ignore_index, scale,
                    int(reduction == 'mean'), int(reduction == 'none'), _p(grad), _p(x_pack), _p(w_pack), _p(lse),
-                   _p(count), _p(o), _p(dx), _p(dw), _p(_buffer(wsb, dev)), wsb, _stream())
+                   _p(count), _p(o), _p(dx), _p(dw), _p(_buffer(wsb, dev)), wsb, _stream_of(dev))
         return dx, dw, None, None, None, None
 
 
@@ -1329,8 +1348,8 @@ def quantize_rows(x):
     with _on(xs.device):
         q = torch.empty(n, ldq, dtype=torch.int8, device=xs.device)
         scale = torch.empty(n, dtype=torch.float32, device=xs.device)
-        L.call('igr_quantize_rows', dt, n, k, _p(xs), ldx, _p(q), ldq, _p(scale), _stream())
-    return q[:, :k], scale
+        L.call('igr_quantize_rows', dt, n, k, _p(xs), ldx, _p(q), ldq, _p(scale), _stream_of(xs.device))
+    return (q if ldq == k else q[:, :k]), scale
 
 
 def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):
@@ -1360,7 +1379,7 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):
     with _on(a.device):
         c = torch.empty(m, n, dtype=out_dtype, device=a.device)
         L.call('igr_gemm_int8', m, n, k, _p(a), lda, _p(a_scale.contiguous()), _p(b), ldb, _p(b_scale.contiguous()),
-               _DTYPES[out_dtype], _p(c), n, _stream())
+               _DTYPES[out_dtype], _p(c), n, _stream_of(a.device))
     return c
 
 
@@ -1388,7 +1407,7 @@ def newton_schulz(g, steps=5, coeffs=NEWTON_SCHULZ_COEFFS, eps=1e-7):
         wsb = L.lib().igr_newton_schulz_workspace_size(b, r, c)
         ws = _buffer(wsb, x.device) if wsb else None
         L.call('igr_newton_schulz', _DTYPES[x.dtype], b, r, c, _p(x), max(x.stride(1), c), x.stride(0), int(steps),
-               *(float(v) for v in coeffs), float(eps), _p(out), _p(ws), wsb, _stream())
+               *(float(v) for v in coeffs), float(eps), _p(out), _p(ws), wsb, _stream_of(x.device))
     return out.view(g.shape)
 
 

@@ -20,6 +20,13 @@ counters, an unsharded trainer on a ROCm device); True insists on it wherever th
 device sampler runs, False always steps eagerly.  The epoch loss is accumulated
 on the device and read once per epoch (the reference syncs with loss.item()
 every step, trainer.py:556).
+
+'loss': 'bpr' (default, the reference's) or 'softmax', the cross entropy of each user's positive
+item against the whole catalogue at 'temperature' (default 1; model.softmax_loss) in place of the
+sampled BPR term, with the same l2 and aux terms beside it.  'score_dtype': 'float32'
+(default) or 'int8', evals ranked from 8-bit user and item rows (ops.quantize_rows once per eval,
+ops.gemm_int8 per batch).  'optimizer': 'Adam', or 'Muon' with 'orthogonal_lr' (default 0.02) for the
+weights of dense layers.
 """
 import contextlib
 import ctypes
@@ -38,7 +45,7 @@ from . import _lib as L
 from . import ops
 from .dataset import AuxiliaryDataset, BPRBatchSampler
 from .model import batch_rep_pays
-from .optim import Adam  # noqa: F401  fused HIP Adam, resolved by name 'Adam'
+from .optim import Adam, Muon  # noqa: F401  resolved by name
 from .sampler import DeviceBPRSampler
 
 
@@ -171,10 +178,31 @@ class BasicTrainer:
         # True while train() runs (or when the caller vouches that train / val / test lists stay
         # as they are): eval() then reuses the exclusion CSR and the metric keys between calls
         self.static_eval_lists = trainer_config.get('static_eval_lists', False)
+        self.score_dtype = trainer_config.get('score_dtype', 'float32')
+        if self.score_dtype not in ('float32', 'int8'):
+            raise ValueError(f"score_dtype {self.score_dtype!r}: 'float32' or 'int8'")
+        if self.score_dtype == 'int8' and torch.device(self.device).type != 'cuda':
+            raise ValueError('int8 scores need a ROCm device')
 
     def initialize_optimizer(self):
         opt = getattr(sys.modules[__name__], self.config['optimizer'])
-        self.opt = opt(self.model.parameters(), lr=self.config['lr'])
+        if hasattr(opt, 'for_model'):  # Muon: which parameters are dense weights is the model's to say
+            self.opt = opt.for_model(self.model, lr=self.config['lr'], orthogonal_lr=self.config.get('orthogonal_lr', 0.02))
+        else:
+            self.opt = opt(self.model.parameters(), lr=self.config['lr'])
+
+    def initialize_loss(self):
+        """The main loss term of a trainer that has the choice ('loss', 'temperature')."""
+        self.loss = self.config.get('loss', 'bpr')
+        temperature = float(self.config.get('temperature', 1.0))
+        if self.loss not in ('bpr', 'softmax'):
+            raise ValueError(f"loss {self.loss!r}: 'bpr' or 'softmax'")
+        if self.loss == 'softmax':
+            if not temperature > 0 or not np.isfinite(temperature):
+                raise ValueError(f'temperature {temperature}: positive and finite')
+            if not self.fused:
+                raise ValueError("loss 'softmax' has no unfused form")
+        self.loss_scale = 1.0 / temperature
 
     def train_one_epoch(self):
         raise NotImplementedError
@@ -316,6 +344,7 @@ class BasicTrainer:
                              self.dataset.train_data, self.dataset.val_data)
             excl = cache[ck]
         kmax = max(self.topks)
+        predict = self._int8_predict(rep) if self.score_dtype == 'int8' else self.model.predict
         rec = []
         # test_batch_size bounds the reference's score matrix; rows are ranked
         # independently, so a batch sized for HBM (~1 GB of scores) gives the same
@@ -325,7 +354,7 @@ class BasicTrainer:
         for s in range(0, n_users, batch):
             e = min(n_users, s + batch)
             users = torch.arange(s, e, dtype=torch.int64, device=self.device)
-            scores = self.model.predict(users, rep)
+            scores = predict(users, rep)
             if excl is not None:
                 ops.mask_scores(scores, excl[0][s:e + 1], excl[1])
             if banned_items is not None:
@@ -334,6 +363,15 @@ class BasicTrainer:
             rec.append(items)  # stays on the device: one copy (and sync) per eval, not per batch
         rec = torch.cat(rec)
         return rec.cpu().numpy() if to_host else rec
+
+    def _int8_predict(self, rep):
+        """model.predict from the 8-bit rows of rep, quantised here once."""
+        q, scale = ops.quantize_rows(rep)
+        items = self.model.n_users
+
+        def predict(users, _):
+            return ops.gemm_int8(q[users], scale[users], q[items:], scale[items:])
+        return predict
 
     def eval(self, val_or_test, banned_items=None):
         """trainer.py:146-210; returns the reference's triple (result string,
@@ -435,7 +473,7 @@ class StepGraph:
         that stream just before the batch's first use (BasicModel._join_batch_stream).  The
         batch-row step reads the batch first; other trainers never join."""
         tr, model = self.tr, self.tr.model
-        if not getattr(tr, 'fused', False) or not hasattr(model, 'bpr_loss') or \
+        if not getattr(tr, 'fused', False) or getattr(tr, 'loss', 'bpr') != 'bpr' or not hasattr(model, 'bpr_loss') or \
                 not hasattr(model, '_join_batch_stream') or model.config.get('draw_stream', True) is False:
             return None
         rows = model._rows_path(n) if hasattr(model, '_rows_path') else batch_rep_pays(model, n)
@@ -597,10 +635,14 @@ class BPRTrainer(BasicTrainer):
         self.initialize_optimizer()
         self.l2_reg = trainer_config['l2_reg']
         self.fused = trainer_config.get('fused', True)
+        self.initialize_loss()
 
     def step(self, users, pos_items, neg_items):
         """One training step on a device batch; returns the loss tensor."""
         self._eager_step_guard()
+        if self.loss == 'softmax':
+            loss, l2 = self.model.softmax_loss(users, pos_items, self.loss_scale, need_l2=self.l2_reg != 0)
+            return fused_loss_step(self, loss, l2)
         if self.fused and hasattr(self.model, 'bpr_loss'):
             bpr_loss, l2 = self.model.bpr_loss(users, pos_items, neg_items, need_l2=self.l2_reg != 0)
             return fused_loss_step(self, bpr_loss, l2)
@@ -643,10 +685,14 @@ class IGCNTrainer(BasicTrainer):
         self.l2_reg = trainer_config['l2_reg']
         self.aux_reg = trainer_config['aux_reg']
         self.fused = trainer_config.get('fused', True)
+        self.initialize_loss()
 
     def step(self, users, pos_items, neg_items, a_users, a_pos, a_neg):
         self._eager_step_guard()
         m = self.model
+        if self.loss == 'softmax':
+            loss, l2 = m.softmax_loss(users, pos_items, self.loss_scale, need_l2=self.l2_reg != 0)
+            return fused_loss_step(self, loss, l2, m.aux_loss(a_users, a_pos, a_neg))
         if self.fused:
             bpr_loss, l2, aux_loss = m.bpr_aux_loss(users, pos_items, neg_items, a_users, a_pos, a_neg,
                                                     need_l2=self.l2_reg != 0)

@@ -107,3 +107,16 @@ def test_newton_schulz_c_arguments():
     assert ns(batch=0) == 0 and ns(rows=0) == 0
     assert lib.igr_newton_schulz_workspace_size(6, 64, 64) == 0  # one workgroup a matrix
     assert lib.igr_newton_schulz_workspace_size(1, 128, 512) == (3 * 128 * 512 + 2 * 128 * 128) * 4 + 256 * 8
+
+
+def test_muon_c_arguments():
+    lib = L.lib()
+    s = (L.IgrMuonSlot * 17)()
+    at = ctypes.addressof(s)
+    for f, tail in ((lib.igr_muon_direction_f32, (0.9, 1)), (lib.igr_muon_apply_f32, (0.1, 0.0, 1.0))):
+        for n, p, msg in ((-1, at, 'n_slots'), (17, at, 'n_slots'), (1, None, 'NULL slots'), (1, at, 'size')):
+            assert f(n, p, *tail, None) == 1 and msg in lib.igr_last_error().decode()
+        s[0].n = 4
+        assert f(1, at, *tail, None) == 1 and 'NULL pointer' in lib.igr_last_error().decode()
+        s[0].n = 0
+        assert f(0, None, *tail, None) == 0
