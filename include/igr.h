@@ -544,11 +544,12 @@ int igr_layer_tail_bwd_f32(int64_t n, int32_t d, const float *gn, int64_t ldgn, 
  * items [v, d] are of `dtype`, unit inner stride, 0 < d <= 256, any alignment; scale > 0.
  *   x_pack, item_pack  igr_softmax_loss_pack_size bytes each, 16-byte aligned: the tables as
  *                      matrix fragments, written here and read by the backward
- *   loss, lse2 [b]     the rows' losses and log2 of the sums
+ *   loss [b]           the rows' losses
+ *   lse2 [2 b]         log2 of the rows' sums, then the softmax weight of all items but the target
  *   total, count       (both or neither) the sum, with `mean` the mean, of the losses over the
  *                      rows that are not ignored (0 if there are none), and their number
  *   o                  [b, 32 / 64 / 128 / 256 - the next that holds d] rows of
- *                      sum_v softmax_bv items_v for dx; NULL if dx will not be asked for
+ *                      sum_v softmax_bv items_v without the target for dx; NULL if dx will not be asked for
  * The workspace holds igr_softmax_loss_workspace_size(b, v, d, 0, o != NULL) bytes.  fp32
  * products run on the 16-bit matrix cores in three parts with fp32's accuracy; half types
  * multiply as they are and round the softmax weights once.  Fixed summation order. */

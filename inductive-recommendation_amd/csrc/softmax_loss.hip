@@ -3,11 +3,13 @@
 //
 //   s_bv   = scale <x_b, w_v>                       b < B batch rows, v < V items, width d <= 256
 //   loss_b = log sum_v exp(s_bv) - s_b,t(b)         0 for rows whose target is ignore_index
-//   dx_b   = c_b (o_b - w_t(b)),  o_b = sum_v p_bv w_v,  p_bv = exp(s_bv - lse_b)
-//   dw_v   = sum_b c_b (p_bv - [v = t(b)]) x_b,     c_b = scale d(total)/d(loss_b)
+//   dx_b   = c_b (o_b - r_b w_t(b)),  o_b = sum_{v != t} p_bv w_v,  p_bv = exp(s_bv - lse_b)
+//   dw_v   = sum_b c_b g_bv x_b,  g_bv = p_bv, at the target -r_b;   c_b = scale d(total)/d(loss_b)
+//   r_b    = sum_{v != t} p_bv = 1 - p_bt, summed without the target: a row that is sure of it keeps
+//            its digits (1 - p would lose them), in the loss (log(1 + r/p)) as in the gradients
 //
-// o_b does not depend on the incoming gradient, so the forward pass computes it along with the
-// running maximum and sum (each tile of logits is used for both and dropped); the backward
+// o_b and r_b do not depend on the incoming gradient, so the forward pass computes them along with
+// the running maximum and sum (each tile of logits is used for both and dropped); the backward
 // recomputes the logits once, for dw.  That is 8 B V d flops in all, where the logits
 // kept would need 6 and B V floats.
 //
@@ -150,13 +152,14 @@ struct FwdArgs {
     Packed x, w;
     const int64_t *target;
     float scale2;  // scale log2(e)
-    float *pm, *pz, *pt, *po;  // partials: [splits][B] max (log2), sum, target logit; [splits][B][DP]
+    float *pm, *pz, *pt, *po;  // partials: [splits][B] max (log2), sum without the target, its logit; [splits][B][DP]
     int32_t *pc;               // [splits] exponent of po
 };
 
 // WITH_O = false: the loss alone (no product with the T part, which is then not copied either).
+// Two workgroups a CU wherever the registers do: all but fp32 rows of 256.
 template <class P, int DP, int NB, bool WITH_O>
-__global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdArgs a) {
+__global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax_fwd(FwdArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32;
     constexpr int TILE = block_halves<P>(DP) / 8 / (WITH_O ? 1 : 2);  // u32x4_t of a streamed block
     constexpr int BLK = block_halves<P>(DP) / 8;
@@ -238,11 +241,15 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             // lane: batch row `col` of block n; register i: item 8 (i/4) + 4 h + i%4
-            const float c = c_x[n] * c_w;
-            if (__any((unsigned)(tgt[n] - v0) < 32u)) {  // some row's target is here: keep its logit
+            // (c of two tables of zeros would round to 0, and 0 times infinity is none)
+            const float c = fmaxf(c_x[n] * c_w, 1.17549435e-38f);
+            if (__any((unsigned)(tgt[n] - v0) < 32u)) {  // some row's target is here: its logit apart from the others
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (tgt[n] - v0 == 8 * (i >> 2) + 4 * h + (i & 3)) tl[n] = acc[n][i] * c;
+                    if (tgt[n] - v0 == 8 * (i >> 2) + 4 * h + (i & 3)) {
+                        tl[n] = acc[n][i] * c;
+                        acc[n][i] = -INFINITY;
+                    }
             }
             if (nv < kRB) {  // the catalogue's last block: its padding takes no part
 #pragma unroll
@@ -255,7 +262,7 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
             if (__any(mx > m[n])) {  // rare after the first blocks
                 const float mn = fmaxf(m[n], mx);
-                const float f = __builtin_amdgcn_exp2f(m[n] - mn);
+                const float f = m[n] == mn ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);  // (both may be -infinity)
                 m[n] = mn;
                 z[n] *= f;
                 if constexpr (WITH_O) {
@@ -270,16 +277,11 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_fwd(FwdA
             // below adds nothing to o either way.
             // (without o the same powers, for the same sums bit for bit)
             const int sh = 14 + (P::kScaled ? max(ew - C, -60) : 0);
-            const float off = m[n] - (float)sh;
+            // (no maximum yet: the target is the only item so far)
+            const float off = m[n] == -INFINITY ? 0.f : m[n] - (float)sh;
             float p[16];
-            if (nv < kRB) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    p[i] = 8 * (i >> 2) + 4 * h + (i & 3) < nv ? __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off)) : 0.f;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
-            }
+            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
             float s0 = 0.f, s1 = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
@@ -346,7 +348,7 @@ struct JoinArgs {
     const int32_t *pc;
     const int64_t *target;
     int64_t ignore;
-    float *loss, *lse2, *o;  // o: [B, DP] or NULL
+    float *loss, *lse2, *rest, *o;  // rest: r; o: [B, DP] or NULL
 };
 
 // One batch row per workgroup: the splits' (max, sum, o) joined in split order, a quarter of them
@@ -362,12 +364,15 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
         if (t == 0) {
             a.loss[b] = 0.f;
             a.lse2[b] = 0.f;
+            a.rest[b] = 0.f;
         }
         if (a.o)
             for (int c = t; c < DP; c += kThreads) a.o[b * DP + c] = 0.f;
         return;
     }
-    float m = -INFINITY;
+    const bool named = tg >= 0 && tg < a.V;
+    const float st = named ? a.pt[(tg / kRB / a.per) * a.B + b] : -INFINITY;
+    float m = st;
     for (int64_t s = t; s < a.splits; s += kThreads) m = fmaxf(m, a.pm[s * a.B + b]);
 #pragma unroll
     for (int q = 32; q; q >>= 1) m = fmaxf(m, __shfl_xor(m, q, 64));
@@ -381,16 +386,19 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
     for (int q = 32; q; q >>= 1) z += __shfl_xor(z, q, 64);
     if (lane == 0) wz[wave] = z;
     __syncthreads();
-    z = (wz[0] + wz[1]) + (wz[2] + wz[3]);
+    const float others = (wz[0] + wz[1]) + (wz[2] + wz[3]);
+    z = others;
+    float loss = NAN;  // a target that names no item
+    if (named) {
+        const float zt = __builtin_amdgcn_exp2f(st - m);
+        z += zt;
+        // terms >= 0 either way, no cancellation
+        loss = st - m > -1.f ? log1pf(others / zt) : kLn2 * (m - st) + logf(z);
+    }
     if (t == 0) {
-        float loss = NAN;  // a target that names no item
-        if (tg >= 0 && tg < a.V) {
-            const float st = a.pt[(tg / kRB / a.per) * a.B + b];
-            loss = kLn2 * (m - st) + logf(z);  // both terms >= 0 up to rounding: no cancellation
-            loss = loss < 0.f ? 0.f : loss;
-        }
         a.loss[b] = loss;
         a.lse2[b] = m + log2f(z);
+        a.rest[b] = others / z;
     }
     if (!a.o) return;
     const int64_t q0 = a.splits * wave / 4, q1 = a.splits * (wave + 1) / 4;
@@ -443,8 +451,8 @@ __global__ __launch_bounds__(kThreads) void softmax_reduce(int64_t B, const floa
 }
 
 // What the streamed batch blocks of the backward carry besides their fragments, per row: the
-// exponent offset that makes exp2(acc c - off) = |c_b| p 2^(14 + e - C), the same power of c_b for
-// the target's own term, the target.
+// exponent offset that makes exp2(acc c - off) = |c_b| p 2^(14 + e - C), the same power of c_b r_b for
+// the target's own term (with c_b's sign, zero or not), the target.
 struct RowInfo {
     float *off, *hot;
     int32_t *tgt;
@@ -455,7 +463,7 @@ struct RowInfo {
 struct CoefArgs {
     int64_t B, V;
     int32_t d, per_row, mean;
-    const float *grad, *count, *lse2, *o;
+    const float *grad, *count, *lse2, *rest, *o;
     const int64_t *target;
     int64_t ignore;
     float scale;
@@ -484,9 +492,10 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
         const int64_t tg = a.target[b];
         const float c = row_coef(a, b, tg);
         const bool ok = tg != a.ignore;
+        const float r = a.rest[b];
         const T *w = static_cast<const T *>(a.items) + (tg >= 0 && tg < a.V ? tg : 0) * a.ld_items;
         T *dx = static_cast<T *>(a.dx) + b * a.d;
-        for (int q = lane; q < a.d; q += 64) dx[q] = ok ? (T)(c * (a.o[b * DP + q] - (float)w[q])) : (T)0.f;
+        for (int q = lane; q < a.d; q += 64) dx[q] = ok ? (T)(c * fmaf(-r, (float)w[q], a.o[b * DP + q])) : (T)0.f;
         return;
     }
     __shared__ int32_t cm;
@@ -504,20 +513,22 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     if (b >= blocks_of(a.B) * kRB) return;
     float off = INFINITY, hot = 0.f;
     int tgt = -1;
+    bool minus = false;
     if (b < a.B) {
         const int64_t tg = a.target[b];
         const float c = row_coef(a, b, tg);
         const int e = SCALED ? a.x.exps[b / kRB] : 0;
         if (c != 0.f) {
             off = a.lse2[b] - log2f(fabsf(c)) - (float)(14 + e - C);
-            hot = ldexpf(c, 14 + e - C);
+            hot = ldexpf(c * a.rest[b], 14 + e - C);
+            minus = c < 0.f;
             tgt = tg >= 0 && tg < a.V ? (int)tg : -1;
         }
     }
     a.info.off[b] = off;
     a.info.hot[b] = hot;
     a.info.tgt[b] = tgt;
-    const uint64_t neg = __ballot(hot < 0.f);
+    const uint64_t neg = __ballot(minus);
     if ((lane & 31) == 0) a.info.neg[b / kRB] = (uint32_t)(neg >> lane) != 0;
     if (b == 0) *a.info.cmax = C;
 }
@@ -547,14 +558,14 @@ __device__ __forceinline__ void store4(T *dst, int c, int d, bool vec, float a, 
     if (c + 3 < d) dst[c + 3] = (T)f;
 }
 
+// (As for the forward, two workgroups a CU but for fp32 rows of 256.)
 // dw of 32 NB items a wave: logits recomputed tile by tile, weights times batch rows accumulated.
 template <class P, int DP, int NB>
-__global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdArgs a) {
+__global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax_bwd(BwdArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32;
     constexpr int BLK = block_halves<P>(DP) / 8;
-    constexpr int NST = (BLK + kThreads - 1) / kThreads;
-    __shared__ u32x4_t lds[2][BLK];
-    __shared__ float info[2][3][kRB];  // off, hot, target of the streamed block
+    __shared__ u32x4_t lds0[BLK], lds1[BLK];
+    __shared__ float info0[3][kRB], info1[3][kRB];  // off, hot, target of the streamed block
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
     const int64_t nvb = blocks_of(a.V), nxb = blocks_of(a.B);
     const int64_t split = blockIdx.y;
@@ -580,86 +591,97 @@ __global__ __launch_bounds__(kThreads, (DP <= 64 ? 2 : 1)) void softmax_bwd(BwdA
             for (int i = 0; i < 16; ++i) o[q][n][i] = 0.f;
     }
 
-    u32x4_t st[NST];
-    float si = 0.f;
-    auto fetch = [&](int64_t k) {
-        const u32x4_t *src = a.x.blocks + k * BLK;
-#pragma unroll
-        for (int i = 0; i < NST; ++i)
-            if (BLK % kThreads == 0 || i * kThreads + t < BLK) st[i] = src[i * kThreads + t];
-        if (t < kRB) si = a.info.off[k * kRB + t];
-        else if (t < 2 * kRB) si = a.info.hot[k * kRB + t - kRB];
-        else if (t < 3 * kRB) si = __builtin_bit_cast(float, a.info.tgt[k * kRB + t - 2 * kRB]);
+    // As in the forward: x and info in use, the next ones filled meanwhile, two arrays by name.
+    auto fetch_info = [&](int64_t k) {
+        float v = 0.f;
+        if (t < kRB) v = a.info.off[k * kRB + t];
+        else if (t < 2 * kRB) v = a.info.hot[k * kRB + t - kRB];
+        else if (t < 3 * kRB) v = __builtin_bit_cast(float, a.info.tgt[k * kRB + t - 2 * kRB]);
+        return v;
     };
-    auto stage = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NST; ++i)
-            if (BLK % kThreads == 0 || i * kThreads + t < BLK) lds[buf][i * kThreads + t] = st[i];
-        if (t < 3 * kRB) info[buf][t / kRB][t % kRB] = si;
-    };
-    fetch(k0);
-    stage(0);
-    __syncthreads();
-    int buf = 0;
-    for (int64_t k = k0; k < k1; ++k, buf ^= 1) {
-        if (k + 1 < k1) fetch(k + 1);
-        const u32x4_t *x = lds[buf];
-        const float c_x = P::kScaled ? pow2f(__builtin_amdgcn_readfirstlane(a.x.exps[k]) - P::kOff) : 1.f;
-        const bool neg = __builtin_amdgcn_readfirstlane(a.info.neg[k]) != 0;
+    int e_next = P::kScaled ? a.x.exps[k0] : 0, neg_next = a.info.neg[k0];
+    auto step = [&](int64_t k, const u32x4_t *__restrict__ x, u32x4_t *__restrict__ next, const float (*info)[kRB],
+                    float (*info_next)[kRB]) {
+        const float c_x = P::kScaled ? pow2f(__builtin_amdgcn_readfirstlane(e_next) - P::kOff) : 1.f;
+        const bool neg = __builtin_amdgcn_readfirstlane(neg_next) != 0;
+        float si = 0.f;
+        if (k + 1 < k1) {
+            if (P::kScaled) e_next = a.x.exps[k + 1];
+            neg_next = a.info.neg[k + 1];
+            si = fetch_info(k + 1);
+            copy_to_lds<BLK>(a.x.blocks + (k + 1) * BLK, next, t);
+        }
         f32x16_t acc[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
-        Frags<P> xf[2];
-        load_frags<P>(x, 0, lane, xf[0]);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            load_frags<P>(x, s + 1, lane, xf[(s + 1) & 1]);
-            mfma_row<P, NB>(xf[s & 1], [&](int n) -> const Frags<P> & { return wf[n][s]; }, acc);
+            Frags<P> xf;
+            load_frags<P>(x, s, lane, xf);
+            mfma_row<P, NB>(xf, [&](int n) -> const Frags<P> & { return wf[n][s]; }, acc);
         }
         // lane: item v0 + col; register i: batch row 8 (i/4) + 4 h + i%4 of the block
-        float off[16];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 f = *reinterpret_cast<const float4 *>(&info[buf][0][8 * g + 4 * h]);
-            off[4 * g] = f.x;
-            off[4 * g + 1] = f.y;
-            off[4 * g + 2] = f.z;
-            off[4 * g + 3] = f.w;
-        }
-        const int tcol = __builtin_bit_cast(int, info[buf][2][col]);
+        const int tcol = __builtin_bit_cast(int, info[2][col]);
         Frags<P> pf[NB][2];
+        Frags<P> rest[NB][P::NS == 1 ? 2 : 1];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const float c = c_w[n] * c_x;
             float p[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off[i]));
+            for (int g = 0; g < 4; ++g) {
+                const float4 off = *reinterpret_cast<const float4 *>(&info[0][8 * g + 4 * h]);
+                p[4 * g] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g], c, -off.x));
+                p[4 * g + 1] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g + 1], c, -off.y));
+                p[4 * g + 2] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g + 2], c, -off.z));
+                p[4 * g + 3] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g + 3], c, -off.w));
+            }
             if (neg) {  // a negative c_b: only where the caller's gradients are
 #pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = copysignf(p[i], info[buf][1][8 * (i >> 2) + 4 * h + (i & 3)]);
+                for (int i = 0; i < 16; ++i) p[i] = copysignf(p[i], info[1][8 * (i >> 2) + 4 * h + (i & 3)]);
             }
             if (__any((unsigned)(tcol - v0[n]) < 32u)) {  // some row's target is one of these items
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (__builtin_bit_cast(int, info[buf][2][r]) == v0[n] + col) p[i] -= info[buf][1][r];
+                    if (__builtin_bit_cast(int, info[2][r]) == v0[n] + col) p[i] = -info[1][r];
                 }
             }
             float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
             float (&ph)[8] = reinterpret_cast<float (&)[8]>(p[8]);
             split8(pl, pf[n][0]);
             split8(ph, pf[n][1]);
+            if constexpr (P::NS == 1) {
+                // Half types: the weight as a pair of them, what the first rounding left as the second.  A
+                // target's term often is nearly all of its item's gradient, and rounded once it took the
+                // gradient's error from 1.7e-3 of its norm, the result's own rounding, to 2.8e-3 (bf16).
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] -= (float)pf[n][i >> 3].p[0][i & 7];
+                split8(pl, rest[n][0]);
+                split8(ph, rest[n][1]);
+            }
         }
 #pragma unroll
         for (int f = 0; f < 2 * DB; ++f) {
-            if (f + 1 < 2 * DB) load_frags<P>(x, KS + f + 1, lane, xf[(KS + f + 1) & 1]);
+            Frags<P> xf;
+            load_frags<P>(x, KS + f, lane, xf);
             f32x16_t (&of)[NB] = o[f >> 1];
-            mfma_row<P, NB>(xf[(KS + f) & 1], [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
+            mfma_row<P, NB>(xf, [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
+            if constexpr (P::NS == 1) mfma_row<P, NB>(xf, [&](int n) -> const Frags<P> & { return rest[n][f & 1]; }, of);
         }
-        if (k + 1 < k1) stage(buf ^ 1);
+        if (k + 1 < k1 && t < 3 * kRB) info_next[t / kRB][t % kRB] = si;
+        copies_done();
         __syncthreads();
+    };
+    copy_to_lds<BLK>(a.x.blocks + k0 * BLK, lds0, t);
+    if (t < 3 * kRB) info0[t / kRB][t % kRB] = fetch_info(k0);
+    copies_done();
+    __syncthreads();
+    for (int64_t k = k0; k < k1; k += 2) {
+        step(k, lds0, lds1, info0, info1);
+        if (k + 1 < k1) step(k + 1, lds1, lds0, info1, info0);
     }
     const float f = a.splits > 1 ? 1.f : ldexpf(1.f, *a.info.cmax - 14 - P::kOff);
 #pragma unroll
@@ -851,7 +873,7 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
                     else hipLaunchKernelGGL((softmax_fwd<P, DP, 1, false>), g, dim3(kThreads), 0, st, a);
                 }
                 JoinArgs j{b, v, a.splits, a.per, d, 14 + P::kOff, a.pm, a.pz, a.pt, a.po, a.pc, target, ignore_index,
-                           loss, lse2, o};
+                           loss, lse2, lse2 + b, o};
                 hipLaunchKernelGGL((softmax_join<DP>), dim3((unsigned)b), dim3(kThreads), 0, st, j);
                 return IGR_OK;
             });
@@ -890,7 +912,7 @@ extern "C" int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t
         a.scale2 = scale * kLog2e;
         a.dw = dw;
         const FwdPlan plan = bwd_plan(b, v, dp);
-        CoefArgs ca{b, v, d, per_row, mean, grad, count, lse2, o, target, ignore_index, scale, a.x, a.info,
+        CoefArgs ca{b, v, d, per_row, mean, grad, count, lse2, lse2 + b, o, target, ignore_index, scale, a.x, a.info,
                     dw ? (blocks_of(b) * kRB + kThreads - 1) / kThreads : 0, items, ld_items, dx};
         const int64_t cg = ca.n_info + (dx ? (b + 3) / 4 : 0);
         if (plan.splits > 65535 || plan.nbt > INT32_MAX) return arg_error(fn, "too many workgroups");

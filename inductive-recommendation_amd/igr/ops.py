@@ -1269,7 +1269,7 @@ class SoftmaxLoss(torch.autograd.Function):
         lib = L.lib()
         with _on(dev):
             packs = [_buffer(lib.igr_softmax_loss_pack_size(n, d, dt), dev) for n in (B, V)]
-            loss, lse = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
+            loss, lse = (torch.empty(n, dtype=torch.float32, device=dev) for n in (B, 2 * B))
             total = count = o = None
             if reduction != 'none':
                 total, count = torch.empty((), device=dev), torch.empty((), device=dev)

@@ -128,6 +128,41 @@ def test_sharp_and_large_logits(dtype):
     check(x, w, w.float().matmul(x.float()[0]).argmax().expand(64).contiguous())  # one item is every row's target
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_rows_that_are_sure_of_their_target_keep_their_digits(dtype):
+    """With p_t = 1 - r and r from 3e-1 down to 1e-7, the loss log(1 + r / p_t) and dx = c (sum_{v != t} p_v w_v -
+    r w_t) are as small as r.  Both are sums without the target, so their error is e (as above, of the
+    terms of these sums), not the fp32 step of 1: relative to r."""
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    V, d, B = 300, 64, 64
+    w = torch.randn(V, d, generator=gen, device=DEV) * 0.3
+    t = torch.randint(0, V, (B,), generator=gen, device=DEV)
+    x = w[t] / w[t].square().sum(1, keepdim=True) * torch.linspace(7, 26, B, device=DEV)[:, None]
+    x, w = x.to(dtype).requires_grad_(), w.to(dtype).requires_grad_()
+    loss = ops.softmax_loss(x, w, t, reduction='none')
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    X, W = x.detach().double(), w.detach().double()
+    s = X.matmul(W.t())
+    at = torch.arange(B, device=DEV)
+    rel = (s - s[at, t][:, None]).exp()
+    rel[at, t] = 0.0
+    ref = torch.log1p(rel.sum(1))
+    p = rel / (1.0 + rel.sum(1, keepdim=True))
+    r = p.sum(1, keepdim=True)
+    assert float(ref.min()) < 1e-6 and float(ref.max()) > 1e-2
+    a = X.abs().matmul(W.abs().t()).amax(1)
+    e = 2 * (3 * d + 16) * 2.0 ** -24 * a + 2.0 ** -20 + 75 * 2.0 ** -24
+    assert ((loss.double() - ref).abs() <= 2 * e * ref + 1e-30).all()
+    half = HALF[dtype]
+    w_round = 0.0 if dtype == torch.float32 else half
+    gx = p.matmul(W) - r * W[t]
+    mx = p.matmul(W.abs()) + r * W[t].abs()
+    # the forward's weights are held from 2^14 at the largest logit, here another item's or the target's
+    floor = (V * 2.0 ** -37 if dtype != torch.bfloat16 else 0.0) * p.amax(1, keepdim=True) * W.abs().max()
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-37
+    assert ((dx.double() - gx).abs() <= (2 * e[:, None] + w_round) * mx + floor + half * gx.abs() + tiny).all()
+
+
 def test_rows_of_very_different_size():
     """Block scales: whole blocks of the tables 2^10 apart, single large rows among small ones."""
     x, w, t = tables(320, 1000, 64, torch.float32, seed=7)
