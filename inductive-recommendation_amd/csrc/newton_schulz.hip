@@ -289,6 +289,8 @@ struct Prod {
     const u32x4_t *add;       // what is added, with d0's layout
     int64_t badd;
     float f_add, f_mul;     // result = f_add add + f_mul product
+    int64_t splits, per;    // of the contraction, in 16-column steps (256-high tiles)
+    float4 *part;
 };
 
 // One 32 x 32 block at (m0, n0): scaled, added to, written both ways.  `turn` is a wave's 32 x 33 floats.
@@ -338,15 +340,20 @@ __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_
 
 // The tile of a workgroup: each XCD (blockIdx % 8) takes a run of consecutive tiles, so that tiles which
 // share operand rows share an L2.  False for the surplus workgroups of the last run.
-template <int MODE>
+// A tile is R times as high as wide.
+__device__ __forceinline__ int64_t tile_id() {
+    return (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+}
+template <int MODE, int R>
 __device__ __forceinline__ bool tile_of(const Prod &a, int64_t &m, int64_t &n) {
-    const int64_t id = (int64_t)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int64_t id = tile_id();
     if (id >= a.tiles) return false;
-    if constexpr (MODE == kGram || MODE == kPoly) {  // tiles on and below the diagonal, row by row
-        m = (int64_t)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
-        while (m * (m + 1) / 2 > id) --m;
-        while ((m + 1) * (m + 2) / 2 <= id) ++m;
-        n = id - m * (m + 1) / 2;
+    if constexpr (MODE == kGram || MODE == kPoly) {  // tiles that reach the diagonal or below, row by row
+        auto before = [](int64_t row) { return R * row * (row + 1) / 2; };
+        m = (int64_t)((sqrtf(8.f / R * (float)id + 1.f) - 1.f) * 0.5f);
+        while (before(m) > id) --m;
+        while (before(m + 1) <= id) ++m;
+        n = id - before(m);
     } else {  // column by column
         m = id % a.tm;
         n = id / a.tm;
@@ -362,7 +369,7 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int64_t batch = blockIdx.y;
     int64_t tm, tn;
-    if (!tile_of<MODE>(a, tm, tn)) return;
+    if (!tile_of<MODE, 1>(a, tm, tn)) return;
     const u32x4_t *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
     f32x16_t acc[BT][BT];
 #pragma unroll
@@ -409,30 +416,32 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
                   reinterpret_cast<float (*)[33]>(&part[wave * (BT == 1 ? 2 : 1)][0][0][0]), lane);
 }
 
-// Many tiles: 128 x 128 a workgroup, four waves of 64 x 64, two 16-column steps at a time.  The rows'
-// operand goes through double-buffered LDS (one barrier each), the columns' straight to registers, a
-// stage ahead: with both in LDS its reads and writes, 128 bytes a clock and CU at the full MFMA rate, were
-// all that LDS gives; like this LDS gives 64 and the vector cache 43.
+// Many tiles: 256 x 128 a workgroup, four waves of 128 x 64 (one a SIMD, half the register file in
+// sums), two 16-column steps at a time.  The rows' operand goes through double-buffered LDS (one
+// barrier a stage), the columns' straight to registers a stage ahead.  A wave's 24 MFMAs a step need 12 KB
+// of operands: 43 bytes a clock and CU from LDS and 21 into it, 43 from the vector cache; 64 x 64
+// waves needed all that LDS (128) or the cache (64) gives and ran at 45 % of the MFMA rate.
+// With fewer tiles than CUs the contraction is split as well, into partial sums that ns_join adds.
 template <int MODE, class T>
-__global__ __launch_bounds__(kThreads, 2) void ns_prod128(Prod a, Mat out, T *y) {
-    constexpr int ST = 4 * 2 * 2 * 64;  // 16-byte groups of a stage: 4 row blocks, 2 steps, 2 planes
+__global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y) {
+    constexpr int ST = 8 * 2 * 2 * 64;  // 16-byte groups of a stage: 8 row blocks, 2 steps, 2 planes
     __shared__ u32x4_t lds[2][ST];
-    __shared__ float turn[4][32][33];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
-    const int64_t batch = blockIdx.y;
+    const int64_t batch = blockIdx.y / a.splits, split = blockIdx.y % a.splits;
     int64_t tm, tn;
-    if (!tile_of<MODE>(a, tm, tn)) return;
+    if (!tile_of<MODE, 2>(a, tm, tn)) return;
+    const int64_t k0 = split * a.per, k1 = k0 + a.per < a.KS ? k0 + a.per : a.KS;
     // thread t stages 16 bytes of each row block: 256 threads are the block's 2 steps of 2 planes
-    const u32x4_t *p = a.p + batch * a.bp + tm * 4 * a.KS * 128 + t;
+    const u32x4_t *p = a.p + batch * a.bp + tm * 8 * a.KS * 128 + t;
     const u32x4_t *q = a.q + batch * a.bq;
-    u32x4_t sp[4];
+    u32x4_t sp[8];
     auto fetch = [&](int64_t k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sp[i] = p[(i * a.KS + k) * 128];
+        for (int i = 0; i < 8; ++i) sp[i] = p[(i * a.KS + k) * 128];
     };
     auto stage = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lds[buf][i * 256 + t] = sp[i];
+        for (int i = 0; i < 8; ++i) lds[buf][i * 256 + t] = sp[i];
     };
     auto columns = [&](int64_t k, Frag2 (&f)[2][2]) {
 #pragma unroll
@@ -440,67 +449,119 @@ __global__ __launch_bounds__(kThreads, 2) void ns_prod128(Prod a, Mat out, T *y)
 #pragma unroll
             for (int i = 0; i < 2; ++i) load2(q, (tn * 4 + wn * 2 + i) * a.KS + k + s, lane, f[s][i]);
     };
-    f32x16_t acc[2][2];
+    f32x16_t acc[4][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i >> 1][i & 1][r] = 0.f;
     Frag2 f0[2][2], f1[2][2];
-    fetch(0);
-    columns(0, f0);
+    fetch(k0);
+    columns(k0, f0);
     stage(0);
     __syncthreads();
     auto step = [&](int64_t k, int buf, Frag2 (&now)[2][2], Frag2 (&next)[2][2]) {
-        const bool more = k + 2 < a.KS;
+        const bool more = k + 2 < k1;
         if (more) {
             fetch(k + 2);
             columns(k + 2, next);
         }
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            Frag2 fp[2];
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) load2(lds[buf], (wm * 2 + i) * 2 + s, lane, fp[i]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                mfma_row<SplitF32, 2>(fp[i], [&](int n) -> const Frag2 & { return now[s][n]; }, acc[i]);
-        }
+            for (int i = 0; i < 4; ++i) {
+                Frag2 fp;
+                load2(lds[buf], (wm * 4 + i) * 2 + s, lane, fp);
+                mfma_row<SplitF32, 2>(fp, [&](int n) -> const Frag2 & { return now[s][n]; }, acc[i]);
+            }
         if (more) stage(buf ^ 1);
         __syncthreads();
     };
-    for (int64_t k = 0; k < a.KS; k += 4) {  // KS is a multiple of 8
+    for (int64_t k = k0; k < k1; k += 4) {  // KS and per are multiples of 4
         step(k, 0, f0, f1);
         step(k + 2, 1, f1, f0);
     }
-    const bool mirror = MODE == kUpdate || tm != tn;
+    if (a.splits > 1) {
+        float4 *d = a.part + (((batch * a.splits + split) * a.tiles + tile_id()) * 4 + wave) * 8 * 256 + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        emit<MODE, T>(a, out, y, batch, (tm * 4 + wm * 2 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32, mirror,
-                      acc[i >> 1][i & 1], turn[wave], lane);
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                d[(i * 4 + g) * 64] = make_float4(acc[i >> 1][i & 1][4 * g], acc[i >> 1][i & 1][4 * g + 1],
+                                                  acc[i >> 1][i & 1][4 * g + 2], acc[i >> 1][i & 1][4 * g + 3]);
+        return;
+    }
+    const bool mirror = MODE == kUpdate || tn < 2 * tm;  // a square's own tiles hold both its triangles
+    float(*turn)[33] = reinterpret_cast<float(*)[33]>(reinterpret_cast<float *>(&lds[0][0]) + wave * 32 * 33);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        emit<MODE, T>(a, out, y, batch, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32, mirror,
+                      acc[i >> 1][i & 1], turn, lane);
+}
+
+// The splits' partial sums in split order, then as above.
+template <int MODE, class T>
+__global__ __launch_bounds__(kThreads) void ns_join(Prod a, Mat out, T *y) {
+    __shared__ float turn[4][32][33];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
+    const int64_t batch = blockIdx.y;
+    int64_t tm, tn;
+    if (!tile_of<MODE, 2>(a, tm, tn)) return;
+    const int i = blockIdx.z;  // one block of each wave's eight
+    f32x16_t s;
+    for (int64_t k = 0; k < a.splits; ++k) {
+        const float4 *d = a.part + (((batch * a.splits + k) * a.tiles + tile_id()) * 4 + wave) * 8 * 256 + lane;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 v = d[(i * 4 + g) * 64];
+            s[4 * g] = k ? s[4 * g] + v.x : v.x;
+            s[4 * g + 1] = k ? s[4 * g + 1] + v.y : v.y;
+            s[4 * g + 2] = k ? s[4 * g + 2] + v.z : v.z;
+            s[4 * g + 3] = k ? s[4 * g + 3] + v.w : v.w;
+        }
+    }
+    emit<MODE, T>(a, out, y, batch, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32,
+                  MODE == kUpdate || tn < 2 * tm, s, turn[wave], lane);
 }
 
 // ------------------------------------------------------------------ host side
 
 struct Plan {
     bool small;
-    int tile;
-    int64_t Sp, Lp, xsz, asz, bytes;
+    int tile;            // rows of a tile: 256 (128 wide), 64 or 32 (square)
+    int64_t Sp, Lp, xsz, asz, splits_gram, splits_poly, part, bytes;
 };
 
 inline int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+inline int64_t tri_tiles(const Plan &p) {  // tiles of a symmetric product that reach the diagonal or below
+    const int64_t n = p.Sp / p.tile;
+    return p.tile == 256 ? n * (n + 1) : n * (n + 1) / 2;
+}
 
 inline Plan plan_of(int64_t batch, int64_t S, int64_t L) {
     Plan p{};
     p.small = S <= 64 && L <= 256;
     if (p.small) return p;
-    // 128-wide tiles once the update has enough of them for half the chip, 64-wide ones for a quarter
-    auto tiles = [&](int64_t t) { return ((S + t - 1) / t) * ((L + t - 1) / t) * batch; };
-    p.tile = tiles(128) >= 128 ? 128 : tiles(64) >= 256 ? 64 : 32;
+    // the largest tiles once the update has enough of them for a good part of the chip and they are
+    // not mostly padding, 64-wide ones once there are 256
+    auto tiles = [&](int64_t h, int64_t w) { return ((S + h - 1) / h) * ((L + w - 1) / w) * batch; };
+    const bool filled = 4 * up_to(S, 256) * up_to(L, 128) <= 5 * S * L;
+    p.tile = filled && tiles(256, 128) >= 96 ? 256 : tiles(64, 64) >= 256 ? 64 : 32;
     p.Sp = up_to(S, p.tile);
-    p.Lp = up_to(L, p.tile);
-    p.xsz = p.Sp * p.Lp / 4;  // u32x4_t: 4 bytes an element
+    p.Lp = up_to(L, p.tile == 256 ? 128 : p.tile);
+    p.xsz = p.Sp * p.Lp / 4;  // 16-byte groups: 4 bytes an element
     p.asz = p.Sp * p.Sp / 4;
-    p.bytes = batch * (3 * p.xsz + 2 * p.asz) * 16 + batch * kSumBlocks * 8;
+    p.splits_gram = p.splits_poly = 1;
+    if (p.tile == 256) {
+        // one workgroup a CU: as many splits as keep to 256 of them, 512 columns each at least
+        auto splits = [&](int64_t K) {
+            return std::max<int64_t>(1, std::min<int64_t>(256 / (tri_tiles(p) * batch), K / 512));
+        };
+        p.splits_gram = splits(p.Lp);
+        p.splits_poly = splits(p.Sp);
+        const int64_t most = std::max(p.splits_gram, p.splits_poly);
+        p.part = most > 1 ? batch * most * tri_tiles(p) * 256 * 128 / 4 : 0;
+    }
+    p.bytes = batch * (3 * p.xsz + 2 * p.asz) * 16 + p.part * 16 + batch * kSumBlocks * 8;
     return p;
 }
 
@@ -523,31 +584,44 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
     w.xt[1] = c, c += batch * p.xsz;
     w.a = c, c += batch * p.asz;
     w.q = c, c += batch * p.asz;
+    float4 *partial = reinterpret_cast<float4 *>(c);
+    c += p.part;
     double *part = reinterpret_cast<double *>(c);
     w.bx = p.xsz, w.ba = p.asz, w.Sp = p.Sp, w.Lp = p.Lp;
     const unsigned nb = (unsigned)batch;
     hipLaunchKernelGGL((ns_sumsq<T>), dim3(kSumBlocks, nb), dim3(kThreads), 0, st, in, src, part);
     const int64_t blocks = (p.Sp / 32) * (p.Lp / 32);
     hipLaunchKernelGGL((ns_pack<T>), dim3((unsigned)((blocks + 3) / 4), nb), dim3(kThreads), 0, st, in, src, part, eps, w);
-    const int64_t ts = p.Sp / p.tile, tl = p.Lp / p.tile;
-    const int64_t tri = ts * (ts + 1) / 2, all = ts * tl;
+    const int64_t ts = p.Sp / p.tile, tl = p.Lp / (p.tile == 256 ? 128 : p.tile);
+    const int64_t tri = tri_tiles(p), all = ts * tl;
     const int64_t ks = p.Sp / 16, kl = p.Lp / 16;
-    auto go = [&](auto mode, const Prod &a) {
-        const unsigned n = (unsigned)((a.tiles + 7) / 8 * 8);
+    auto go = [&](auto mode, Prod a, int64_t splits) {
         constexpr int M = decltype(mode)::value;
-        if (p.tile == 128) hipLaunchKernelGGL((ns_prod128<M, T>), dim3(n, nb), dim3(kThreads), 0, st, a, out, dst);
-        else if (p.tile == 64) hipLaunchKernelGGL((ns_prod_split<M, T, 2, 4>), dim3(n, nb), dim3(256), 0, st, a, out, dst);
-        else hipLaunchKernelGGL((ns_prod_split<M, T, 1, 8>), dim3(n, nb), dim3(512), 0, st, a, out, dst);
+        const unsigned n = (unsigned)((a.tiles + 7) / 8 * 8);
+        a.per = up_to((a.KS + splits - 1) / splits, 4);
+        a.splits = (a.KS + a.per - 1) / a.per;
+        a.part = partial;
+        if (p.tile == 256) {
+            hipLaunchKernelGGL((ns_prod256<M, T>), dim3(n, nb * (unsigned)a.splits), dim3(kThreads), 0, st, a, out, dst);
+            if (a.splits > 1)
+                hipLaunchKernelGGL((ns_join<M, T>), dim3(n, nb, 8), dim3(kThreads), 0, st, a, out, dst);
+        } else if (p.tile == 64) {
+            hipLaunchKernelGGL((ns_prod_split<M, T, 2, 4>), dim3(n, nb), dim3(256), 0, st, a, out, dst);
+        } else {
+            hipLaunchKernelGGL((ns_prod_split<M, T, 1, 8>), dim3(n, nb), dim3(512), 0, st, a, out, dst);
+        }
     };
     for (int32_t s = 0; s < steps; ++s) {
         u32x4_t *cur = w.xt[s & 1], *nxt = w.xt[(s + 1) & 1];
         go(std::integral_constant<int, kGram>(),
-           Prod{w.x, w.x, w.bx, w.bx, kl, tri, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f});
+           Prod{w.x, w.x, w.bx, w.bx, kl, tri, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f, 1, 0, nullptr},
+           p.splits_gram);
         go(std::integral_constant<int, kPoly>(),
-           Prod{w.a, w.a, w.ba, w.ba, ks, tri, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc});
-        const Prod u{w.q, cur, w.ba, w.bx, ks, all, ts, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f};
-        if (s + 1 < steps) go(std::integral_constant<int, kUpdate>(), u);
-        else go(std::integral_constant<int, kLast>(), u);
+           Prod{w.a, w.a, w.ba, w.ba, ks, tri, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc, 1, 0, nullptr},
+           p.splits_poly);
+        const Prod u{w.q, cur, w.ba, w.bx, ks, all, ts, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f, 1, 0, nullptr};
+        if (s + 1 < steps) go(std::integral_constant<int, kUpdate>(), u, 1);
+        else go(std::integral_constant<int, kLast>(), u, 1);
     }
     return launch_status(fn);
 }
@@ -676,7 +750,8 @@ extern "C" int igr_newton_schulz(int32_t dtype, int64_t batch, int64_t rows, int
             return arg_error(fn, "too large: at most 65535 matrices, sides of 2^24, the shorter 2^15");
         const int64_t S = std::min(rows, cols), L = std::max(rows, cols);
         const Plan p = plan_of(batch, S, L);
-        if (!p.small && p.Sp / 32 * (p.Lp / 32) / 4 > INT32_MAX) return arg_error(fn, "too many tiles");
+        if (!p.small && (p.Sp / 32 * (p.Lp / 32) / 4 > INT32_MAX || batch * std::max(p.splits_gram, p.splits_poly) > 65535))
+            return arg_error(fn, "too many tiles");
         if (!g || !out) return arg_error(fn, "null pointer");
         if (p.bytes > 0 && (!workspace || ws_bytes < p.bytes || !aligned16(workspace)))
             return arg_error(fn, "workspace too small or not 16-byte aligned");
