@@ -434,16 +434,17 @@ __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y)
     // thread t stages 16 bytes of each row block: 256 threads are the block's 2 steps of 2 planes
     const u32x4_t *p = a.p + batch * a.bp + tm * 8 * a.KS * 128 + t;
     const u32x4_t *q = a.q + batch * a.bq;
-    u32x4_t sp[8];
-    auto fetch = [&](int64_t k) {
+    auto fetch = [&](int64_t k, u32x4_t (&sp)[8]) {
+        k = k < k1 ? k : k1 - 2;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sp[i] = p[(i * a.KS + k) * 128];
     };
-    auto stage = [&](int buf) {
+    auto stage = [&](int buf, const u32x4_t (&sp)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) lds[buf][i * 256 + t] = sp[i];
     };
     auto columns = [&](int64_t k, Frag2 (&f)[2][2]) {
+        k = k < k1 ? k : k1 - 2;
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -454,31 +455,43 @@ __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y)
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i >> 1][i & 1][r] = 0.f;
-    Frag2 f0[2][2], f1[2][2];
-    fetch(k0);
+    // A stage's loads are given three stages to arrive (the columns' to their registers, the rows' two
+    // to registers and one in LDS).  Past the end the last stage is loaded again: a load under a condition
+    // would make the compiler wait for all loads at each use.
+    u32x4_t s0[8], s1[8];
+    Frag2 f0[2][2], f1[2][2], f2[2][2], f3[2][2];
+    fetch(k0, s0);
+    fetch(k0 + 2, s1);
     columns(k0, f0);
-    stage(0);
+    columns(k0 + 2, f1);
+    columns(k0 + 4, f2);
+    stage(0, s0);
+    fetch(k0 + 4, s0);
     __syncthreads();
-    auto step = [&](int64_t k, int buf, Frag2 (&now)[2][2], Frag2 (&next)[2][2]) {
-        const bool more = k + 2 < k1;
-        if (more) {
-            fetch(k + 2);
-            columns(k + 2, next);
-        }
+    auto step = [&](int64_t k, int buf, u32x4_t (&sp)[8], Frag2 (&now)[2][2], Frag2 (&ahead)[2][2]) {
+        stage(buf ^ 1, sp);
+        fetch(k + 6, sp);
+        columns(k + 6, ahead);
+        // all of the stage's LDS reads first, so that they arrive while the MFMAs run: read right before
+        // its use, as the compiler orders it, each fragment cost its latency (130 us an update instead of UPD)
+        Frag2 fp[2][4];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                Frag2 fp;
-                load2(lds[buf], (wm * 4 + i) * 2 + s, lane, fp);
-                mfma_row<SplitF32, 2>(fp, [&](int n) -> const Frag2 & { return now[s][n]; }, acc[i]);
-            }
-        if (more) stage(buf ^ 1);
+            for (int i = 0; i < 4; ++i) load2(lds[buf], (wm * 4 + i) * 2 + s, lane, fp[s][i]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                mfma_row<SplitF32, 2>(fp[s][i], [&](int n) -> const Frag2 & { return now[s][n]; }, acc[i]);
         __syncthreads();
     };
-    for (int64_t k = k0; k < k1; k += 4) {  // KS and per are multiples of 4
-        step(k, 0, f0, f1);
-        step(k + 2, 1, f1, f0);
+    for (int64_t k = k0; k < k1; k += 8) {  // KS and per are multiples of 8
+        step(k, 0, s1, f0, f3);
+        step(k + 2, 1, s0, f1, f0);
+        step(k + 4, 0, s1, f2, f1);
+        step(k + 6, 1, s0, f3, f2);
     }
     if (a.splits > 1) {
         float4 *d = a.part + (((batch * a.splits + split) * a.tiles + tile_id()) * 4 + wave) * 8 * 256 + lane;
@@ -598,7 +611,7 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
     auto go = [&](auto mode, Prod a, int64_t splits) {
         constexpr int M = decltype(mode)::value;
         const unsigned n = (unsigned)((a.tiles + 7) / 8 * 8);
-        a.per = up_to((a.KS + splits - 1) / splits, 4);
+        a.per = up_to((a.KS + splits - 1) / splits, 8);
         a.splits = (a.KS + a.per - 1) / a.per;
         a.part = partial;
         if (p.tile == 256) {
