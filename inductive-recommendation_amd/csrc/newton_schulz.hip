@@ -206,11 +206,21 @@ __global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double 
     while (wide > 1 && wide / 2 >= cols) wide >>= 1;
     const int t = threadIdx.x, across = kThreads / wide;
     double s = 0.;
-    for (int64_t r = (int64_t)blockIdx.x * across + t / wide; r < rows; r += (int64_t)gridDim.x * across)
-        for (int64_t c = t % wide; c < cols; c += wide) {
-            const float v = (float)src[r * ld + c];
+    for (int64_t r = (int64_t)blockIdx.x * across + t / wide; r < rows; r += (int64_t)gridDim.x * across) {
+        const T *row = src + r * ld;
+        int64_t c = t % wide;
+        for (; c + 7 * wide < cols; c += 8 * wide) {  // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)row[c + i * wide];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += (double)v[i] * v[i];
+        }
+        for (; c < cols; c += wide) {
+            const float v = (float)row[c];
             s += (double)v * v;
         }
+    }
 #pragma unroll
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -418,10 +428,11 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
 
 // Many tiles: 256 x 128 a workgroup, four waves of 128 x 64 (one a SIMD, half the register file in
 // sums), two 16-column steps at a time.  The rows' operand goes through double-buffered LDS (one
-// barrier a stage), the columns' straight to registers a stage ahead.  A wave's 24 MFMAs a step need 12 KB
-// of operands: 43 bytes a clock and CU from LDS and 21 into it, 43 from the vector cache; 64 x 64
-// waves needed all that LDS (128) or the cache (64) gives and ran at 45 % of the MFMA rate.
+// barrier a stage), the columns' straight to registers.  A wave's 24 MFMAs a step need 12 KB of
+// operands: 43 bytes a clock and CU from LDS and 21 into it, 43 from the vector cache, of 128 and 64.
 // With fewer tiles than CUs the contraction is split as well, into partial sums that ns_join adds.
+// The update of 2048 x 4096 takes 114 us, 900 TFLOP/s of 16-bit products; the library's fp16 product of
+// 8192^3 reaches 1555 here.
 template <int MODE, class T>
 __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y) {
     constexpr int ST = 8 * 2 * 2 * 64;  // 16-byte groups of a stage: 8 row blocks, 2 steps, 2 planes
@@ -468,24 +479,46 @@ __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y)
     stage(0, s0);
     fetch(k0 + 4, s0);
     __syncthreads();
+    // One wave a SIMD: its own MFMAs have to cover its LDS traffic.  While a step multiplies, the next step's
+    // fragments are read and (in the first step) the next stage written, a few instructions between
+    // MFMAs; the barrier stands between the two steps.
+    Frag2 fp0[4], fp1[4];
+    auto rows = [&](int buf, int s, Frag2 (&f)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) load2(lds[buf], (wm * 4 + i) * 2 + s, lane, f[i]);
+    };
+    auto multiply = [&](const Frag2 (&f)[4], const Frag2 (&g)[2]) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part)  // lo hi, hi lo, hi hi: eight sums apart
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) acc[i][n] = mfma32(f[i].p[part == 0], g[n].p[part == 1], acc[i][n]);
+    };
+    rows(0, 0, fp0);
     auto step = [&](int64_t k, int buf, u32x4_t (&sp)[8], Frag2 (&now)[2][2], Frag2 (&ahead)[2][2]) {
+        rows(buf, 1, fp1);
         stage(buf ^ 1, sp);
         fetch(k + 6, sp);
         columns(k + 6, ahead);
-        // all of the stage's LDS reads first, so that they arrive while the MFMAs run: read right before
-        // its use, as the compiler orders it, each fragment cost its latency (130 us an update instead of UPD)
-        Frag2 fp[2][4];
+        multiply(fp0, now[0]);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) load2(lds[buf], (wm * 4 + i) * 2 + s, lane, fp[s][i]);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                mfma_row<SplitF32, 2>(fp[s][i], [&](int n) -> const Frag2 & { return now[s][n]; }, acc[i]);
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // LDS write
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);  // loads
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
         __syncthreads();
+        rows(buf ^ 1, 0, fp0);
+        multiply(fp1, now[1]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+            __builtin_amdgcn_sched_group_barrier(0x008, 3, 1);
+        }
     };
     for (int64_t k = k0; k < k1; k += 8) {  // KS and per are multiples of 8
         step(k, 0, s1, f0, f3);
