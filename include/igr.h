@@ -22,7 +22,8 @@
  *    dst = `row`), columns = source nodes (DGL src = `column`).  Edge data
  *    (`rhs`) is indexed by EDGE ID; edge id = CSR position unless the graph
  *    carries an `edge_id` permutation (multigraph built from unsorted COO).
- *  - fp32 throughout (the reference computes in float32).
+ *  - fp32 throughout (the reference computes in float32), except where an
+ *    entry point takes a dtype or 8-bit tables.
  */
 #ifndef IGR_H
 #define IGR_H
@@ -559,7 +560,8 @@ int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const v
                          const void *items, int64_t ld_items, const int64_t *target, int64_t ignore_index,
                          float scale, int32_t mean, void *x_pack, void *item_pack, float *loss, float *lse2,
                          float *total, float *count, float *o, void *workspace, int64_t ws_bytes, void *stream);
-/* Its gradients: dx [b, d] and dw [v, d] of `dtype`, contiguous, either NULL.  grad: one
+/* Its gradients: dx [b, d] (needs items and o) and dw [v, d] (needs the packs) of `dtype`,
+ * contiguous, either NULL.  grad: one
  * device float (the total's gradient), or with per_row one per row; `mean` divides by *count.
  * The workspace holds igr_softmax_loss_workspace_size(b, v, d, 1, 0) bytes. */
 int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *items, int64_t ld_items,

@@ -372,12 +372,14 @@ __device__ __forceinline__ bool tile_of(const Prod &a, int64_t &m, int64_t &n) {
 }
 
 // Few tiles: BT x BT blocks a workgroup, the contraction dealt out to its NW waves, which load fragments
-// straight from memory (four steps in flight) and join their sums in LDS in wave order.
+// straight from memory (four steps in flight) and join their sums in LDS in wave order.  A long
+// contraction is dealt out to workgroups first (ns_join_blocks adds theirs).
 template <int MODE, class T, int BT, int NW>
 __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) {
     __shared__ float part[NW][BT * BT][16][64];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int64_t batch = blockIdx.y;
+    const int64_t batch = blockIdx.y / a.splits, split = blockIdx.y % a.splits;
+    const int64_t k0 = split * a.per, k1 = k0 + a.per < a.KS ? k0 + a.per : a.KS;
     int64_t tm, tn;
     if (!tile_of<MODE, 1>(a, tm, tn)) return;
     const u32x4_t *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
@@ -402,9 +404,9 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
             for (int i = 0; i < BT; ++i)
                 mfma_row<SplitF32, BT>(fp[s][i], [&](int n) -> const Frag2 & { return fq[s][n]; }, acc[i]);
     };
-    int64_t k = wave;
-    for (; k + 3 * NW < a.KS; k += 4 * NW) multiply(k, std::integral_constant<int, 4>());
-    for (; k < a.KS; k += NW) multiply(k, std::integral_constant<int, 1>());
+    int64_t k = k0 + wave;
+    for (; k + 3 * NW < k1; k += 4 * NW) multiply(k, std::integral_constant<int, 4>());
+    for (; k < k1; k += NW) multiply(k, std::integral_constant<int, 1>());
 #pragma unroll
     for (int i = 0; i < BT * BT; ++i)
 #pragma unroll
@@ -421,9 +423,42 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
     }
     __syncthreads();
     if (wave >= BT * BT) return;
+    if (a.splits > 1) {
+        float4 *d = a.part + (((batch * a.splits + split) * a.tiles + tile_id()) * BT * BT + wave) * 256 + lane;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) d[g * 64] = make_float4(s[4 * g], s[4 * g + 1], s[4 * g + 2], s[4 * g + 3]);
+        return;
+    }
     const bool mirror = MODE == kUpdate || tm != tn;
     emit<MODE, T>(a, out, y, batch, (tm * BT + wave / BT) * 32, (tn * BT + wave % BT) * 32, mirror, s,
                   reinterpret_cast<float (*)[33]>(&part[wave * (BT == 1 ? 2 : 1)][0][0][0]), lane);
+}
+
+// The workgroups' partial sums in split order, a wave a block.
+__device__ __forceinline__ f32x16_t join_block(const Prod &a, int64_t batch, int64_t block, int64_t blocks, int lane) {
+    f32x16_t s;
+    for (int64_t k = 0; k < a.splits; ++k) {
+        const float4 *d = a.part + (((batch * a.splits + k) * a.tiles + tile_id()) * blocks + block) * 256 + lane;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float4 v = d[g * 64];
+            s[4 * g] = k ? s[4 * g] + v.x : v.x;
+            s[4 * g + 1] = k ? s[4 * g + 1] + v.y : v.y;
+            s[4 * g + 2] = k ? s[4 * g + 2] + v.z : v.z;
+            s[4 * g + 3] = k ? s[4 * g + 3] + v.w : v.w;
+        }
+    }
+    return s;
+}
+
+template <int MODE, class T, int BT>
+__global__ __launch_bounds__(BT * BT * 64) void ns_join_blocks(Prod a, Mat out, T *y) {
+    __shared__ float turn[BT * BT][32][33];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int64_t tm, tn;
+    if (!tile_of<MODE, 1>(a, tm, tn)) return;
+    emit<MODE, T>(a, out, y, blockIdx.y, (tm * BT + wave / BT) * 32, (tn * BT + wave % BT) * 32,
+                  MODE == kUpdate || tm != tn, join_block(a, blockIdx.y, wave, BT * BT, lane), turn[wave], lane);
 }
 
 // Many tiles: 256 x 128 a workgroup, four waves of 128 x 64 (one a SIMD, half the register file in
@@ -544,29 +579,15 @@ __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y)
                       acc[i >> 1][i & 1], turn, lane);
 }
 
-// The splits' partial sums in split order, then as above.
 template <int MODE, class T>
 __global__ __launch_bounds__(kThreads) void ns_join(Prod a, Mat out, T *y) {
     __shared__ float turn[4][32][33];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
-    const int64_t batch = blockIdx.y;
     int64_t tm, tn;
     if (!tile_of<MODE, 2>(a, tm, tn)) return;
     const int i = blockIdx.z;  // one block of each wave's eight
-    f32x16_t s;
-    for (int64_t k = 0; k < a.splits; ++k) {
-        const float4 *d = a.part + (((batch * a.splits + k) * a.tiles + tile_id()) * 4 + wave) * 8 * 256 + lane;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 v = d[(i * 4 + g) * 64];
-            s[4 * g] = k ? s[4 * g] + v.x : v.x;
-            s[4 * g + 1] = k ? s[4 * g + 1] + v.y : v.y;
-            s[4 * g + 2] = k ? s[4 * g + 2] + v.z : v.z;
-            s[4 * g + 3] = k ? s[4 * g + 3] + v.w : v.w;
-        }
-    }
-    emit<MODE, T>(a, out, y, batch, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32,
-                  MODE == kUpdate || tn < 2 * tm, s, turn[wave], lane);
+    emit<MODE, T>(a, out, y, blockIdx.y, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32,
+                  MODE == kUpdate || tn < 2 * tm, join_block(a, blockIdx.y, wave * 8 + i, 32, lane), turn[wave], lane);
 }
 
 // ------------------------------------------------------------------ host side
@@ -597,7 +618,11 @@ inline Plan plan_of(int64_t batch, int64_t S, int64_t L) {
     p.xsz = p.Sp * p.Lp / 4;  // 16-byte groups: 4 bytes an element
     p.asz = p.Sp * p.Sp / 4;
     p.splits_gram = p.splits_poly = 1;
-    if (p.tile == 256) {
+    if (p.tile < 256) {
+        // long rows (X^T X of an embedding table): 2048 columns a workgroup at least, at most one a CU
+        p.splits_gram = std::max<int64_t>(1, std::min<int64_t>(256 / (tri_tiles(p) * batch), p.Lp / 2048));
+        p.part = p.splits_gram > 1 ? batch * p.splits_gram * tri_tiles(p) * p.tile * p.tile / 4 : 0;
+    } else {
         // one workgroup a CU: as many splits as keep to 256 of them, 512 columns each at least
         auto splits = [&](int64_t K) {
             return std::max<int64_t>(1, std::min<int64_t>(256 / (tri_tiles(p) * batch), K / 512));
@@ -652,9 +677,11 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
             if (a.splits > 1)
                 hipLaunchKernelGGL((ns_join<M, T>), dim3(n, nb, 8), dim3(kThreads), 0, st, a, out, dst);
         } else if (p.tile == 64) {
-            hipLaunchKernelGGL((ns_prod_split<M, T, 2, 4>), dim3(n, nb), dim3(256), 0, st, a, out, dst);
+            hipLaunchKernelGGL((ns_prod_split<M, T, 2, 4>), dim3(n, nb * (unsigned)a.splits), dim3(256), 0, st, a, out, dst);
+            if (a.splits > 1) hipLaunchKernelGGL((ns_join_blocks<M, T, 2>), dim3(n, nb), dim3(256), 0, st, a, out, dst);
         } else {
-            hipLaunchKernelGGL((ns_prod_split<M, T, 1, 8>), dim3(n, nb), dim3(512), 0, st, a, out, dst);
+            hipLaunchKernelGGL((ns_prod_split<M, T, 1, 8>), dim3(n, nb * (unsigned)a.splits), dim3(512), 0, st, a, out, dst);
+            if (a.splits > 1) hipLaunchKernelGGL((ns_join_blocks<M, T, 1>), dim3(n, nb), dim3(64), 0, st, a, out, dst);
         }
     };
     for (int32_t s = 0; s < steps; ++s) {

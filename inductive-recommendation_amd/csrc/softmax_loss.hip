@@ -897,7 +897,7 @@ extern "C" int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t
         if (ld_items < d) return arg_error(fn, "leading dimension too small");
         if (!(scale > 0.f) || !std::isfinite(scale)) return arg_error(fn, "scale must be positive and finite");
         if (b == 0 || (!dx && !dw)) return IGR_OK;
-        if (!target || !grad || !x_pack || !item_pack || !lse2 || (mean && !count) || (dx && (!o || !items)))
+        if (!target || !grad || !lse2 || (mean && !count) || (dx && (!o || !items)) || (dw && (!x_pack || !item_pack)))
             return arg_error(fn, "null pointer");
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
         const int dp = pad_width(d);

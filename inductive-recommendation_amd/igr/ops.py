@@ -1281,7 +1281,8 @@ class SoftmaxLoss(torch.autograd.Function):
                    int(reduction == 'mean'), _p(packs[0]), _p(packs[1]), _p(loss), _p(lse), _p(total), _p(count),
                    _p(o), _p(_buffer(wsb, dev)), wsb, _stream_of(dev))
         if need_x or need_w:
-            ctx.save_for_backward(items, target, packs[0], packs[1], lse, count, o)
+            # the packed tables (twice the tables' size) are for the items' gradient alone
+            ctx.save_for_backward(items, target, *(packs if need_w else (None, None)), lse, count, o)
             ctx.args = (dt, B, V, d, scale, ignore_index, reduction)
         return loss if reduction == 'none' else total
 

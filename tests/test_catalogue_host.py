@@ -31,12 +31,12 @@ def test_softmax_loss_c_arguments():
         assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())
     assert fwd(d=257, ldx=257, ldw=257) == 3  # IGR_ERR_UNSUPPORTED
 
-    def bwd(dtype=0, d=8, ldw=8, scale=1.0, grad=p, ws=p, wsb=1 << 40, count=p):
-        return lib.igr_softmax_loss_bwd(dtype, 4, 6, d, p, ldw, p, -100, scale, 1, 0, grad, p, p, p, count, p, p, p, ws, wsb,
+    def bwd(dtype=0, d=8, ldw=8, scale=1.0, grad=p, ws=p, wsb=1 << 40, count=p, pack=p):
+        return lib.igr_softmax_loss_bwd(dtype, 4, 6, d, p, ldw, p, -100, scale, 1, 0, grad, pack, p, p, count, p, p, p, ws, wsb,
                                         None)
 
     for kw, msg in ((dict(dtype=-1), 'dtype'), (dict(ldw=7), 'leading'), (dict(scale=-1.0), 'scale'),
-                    (dict(grad=None), 'null'), (dict(count=None), 'null'), (dict(ws=None), 'workspace'),
+                    (dict(grad=None), 'null'), (dict(count=None), 'null'), (dict(pack=None), 'null'), (dict(ws=None), 'workspace'),
                     (dict(wsb=16), 'workspace')):
         assert bwd(**kw) == 1, kw
         assert msg in lib.igr_last_error().decode(), (kw, lib.igr_last_error())

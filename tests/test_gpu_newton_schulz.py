@@ -56,7 +56,8 @@ def weight(b, r, c, seed=0, scale=1e-3):
 
 SHAPES = [(1, 1, 1), (2, 1, 9), (1, 7, 3), (6, 64, 64), (3, 64, 33), (2, 5, 128), (1, 64, 129), (2, 256, 64), (1, 33, 256),
           (1, 64, 257), (2, 65, 64), (1, 65, 65), (2, 200, 520), (1, 520, 200), (1, 16, 4000), (1, 1000, 130),
-          (1, 1100, 1030), (3, 700, 900), (1, 1030, 3001), (2, 1500, 1100), (1, 2304, 2304), (9, 300, 700)]
+          (1, 1100, 1030), (3, 700, 900), (1, 1030, 3001), (2, 1500, 1100), (1, 2304, 2304), (9, 300, 700), (1, 40981, 64),
+          (2, 33, 9000), (1, 20000, 100), (1, 300000, 8)]
 
 
 @pytest.mark.parametrize('dtype', TYPES)

@@ -328,6 +328,33 @@ def test_changed_tables_between_forward_and_backward_are_refused():
         loss.backward()
 
 
+def test_table_past_32_bits():
+    """2^31 + bytes of item rows (and twice that packed): the last rows are read and their gradients written
+    where they are.  Sixteen rows at the end carry all of the softmax's weight but 1e-6."""
+    V, d, B = 9_000_000, 64, 8
+    gen = torch.Generator(device=DEV).manual_seed(31)
+    w = torch.zeros(V, d, device=DEV)
+    w[-16:] = torch.randn(16, d, generator=gen, device=DEV)
+    w[:, 0] = -1.0
+    w[-16:, 0] = 0.0
+    x = torch.randn(B, d, generator=gen, device=DEV)
+    x[:, 0] = 32.0   # the other nine million: logits of -32
+    t = V - 1 - torch.randint(0, 16, (B,), generator=gen, device=DEV)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.softmax_loss(x, w, t)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    X, W = x.detach().double(), w.detach()[-16:].double()
+    s = torch.cat([X.matmul(W.t()), torch.full((B, 1), -32.0, device=DEV, dtype=torch.float64)
+                   + torch.log(torch.tensor(float(V - 16), device=DEV, dtype=torch.float64))], 1)
+    p = s.softmax(1)[:, :16]
+    at = t - (V - 16)
+    assert abs(float(loss.detach()) - float(torch.nn.functional.cross_entropy(s, at))) < 1e-5
+    p[torch.arange(B, device=DEV), at] -= 1.0
+    assert (dw[-16:].double() - p.t().contiguous().matmul(X) / B).abs().max() < 1e-5 * 32
+    assert dw[:-16].abs().max() < 1e-9 and (dx[:, 1:].double() - p.matmul(W)[:, 1:] / B).abs().max() < 1e-6
+
+
 def test_refusals_on_the_device():
     x, w, t = tables(4, 6, 8, torch.float32)
     with pytest.raises(IgrError, match='share'):
