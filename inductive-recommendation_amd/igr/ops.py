@@ -14,6 +14,7 @@ DGL-compatible surface (the reference's operator API):
 """
 import contextlib
 import ctypes
+import functools
 import weakref
 import math
 
@@ -1256,53 +1257,70 @@ def _buffer(nbytes, device):
 SOFTMAX_LOSS_MAX_WIDTH = 256
 
 
+@functools.lru_cache(maxsize=64)
+def _softmax_layout(B, V, d, dt, need_x, need_w):
+    """Byte offsets of what a softmax_loss node holds until its backward - lse [2 B], count, o [B, width] and the
+    packed tables, each None if not wanted there - in one buffer, then that buffer's size, the offsets of
+    packs that the forward alone needs in its workspace, and both workspaces' sizes."""
+    lib = L.lib()
+    size = {'lse': 8 * B, 'count': 4, 'o': 4 * B * next(w for w in (32, 64, 128, 256) if w >= d) if need_x else 0,
+            'x_pack': lib.igr_softmax_loss_pack_size(B, d, dt), 'w_pack': lib.igr_softmax_loss_pack_size(V, d, dt)}
+    at, end = {}, 0
+    kept = ('lse', 'count') + (('o',) if need_x else ()) + (('x_pack', 'w_pack') if need_w else ())
+    for k in kept:
+        at[k], end = end, end + (size[k] + 255) // 256 * 256
+    fwd = (lib.igr_softmax_loss_workspace_size(B, V, d, 0, int(need_x)) + 255) // 256 * 256
+    packs = (0, 0) if need_w else (fwd, fwd + (size['x_pack'] + 255) // 256 * 256)
+    total = fwd if need_w else packs[1] + size['w_pack']
+    return at, end, packs, fwd, total, lib.igr_softmax_loss_workspace_size(B, V, d, 1, 0)
+
+
 class SoftmaxLoss(torch.autograd.Function):
     """softmax_loss's node: the packed tables, the log-sums and the softmax-weighted item rows of the
-    forward are all that the backward needs besides one recomputation of the logits."""
+    forward are all that the backward needs besides one recomputation of the logits.  They share a
+    buffer: the backward runs on autograd's own thread, where each Python object costs several times more."""
 
     @staticmethod
     def forward(ctx, x, items, target, scale, ignore_index, reduction):
-        xs, ldx, dt = _table(x, 'softmax_loss x')
-        ws, ldw, _ = _table(items, 'softmax_loss items')
-        (B, d), V, dev = xs.shape, ws.shape[0], xs.device
+        x, ldx, dt = _table(x, 'softmax_loss x')
+        items, ldw, _ = _table(items, 'softmax_loss items')
+        (B, d), V, dev = x.shape, items.shape[0], x.device
         need_x, need_w = ctx.needs_input_grad[:2]
-        lib = L.lib()
+        at, held, packs, wsb, total_ws, bwd_ws = _softmax_layout(B, V, d, dt, need_x, need_w)
         with _on(dev):
-            packs = [_buffer(lib.igr_softmax_loss_pack_size(n, d, dt), dev) for n in (B, V)]
-            loss, lse = (torch.empty(n, dtype=torch.float32, device=dev) for n in (B, 2 * B))
-            total = count = o = None
-            if reduction != 'none':
-                total, count = torch.empty((), device=dev), torch.empty((), device=dev)
-            if need_x:
-                width = next(w for w in (32, 64, 128, 256) if w >= d)
-                o = torch.empty(B, width, dtype=torch.float32, device=dev)
-            wsb = lib.igr_softmax_loss_workspace_size(B, V, d, 0, int(need_x))
-            L.call('igr_softmax_loss_fwd', dt, B, V, d, _p(xs), ldx, _p(ws), ldw, _p(target), ignore_index, scale,
-                   int(reduction == 'mean'), _p(packs[0]), _p(packs[1]), _p(loss), _p(lse), _p(total), _p(count),
-                   _p(o), _p(_buffer(wsb, dev)), wsb, _stream_of(dev))
+            buf, ws = _buffer(held, dev), _buffer(total_ws, dev)
+            base, wbase = buf.data_ptr(), ws.data_ptr()
+            # the packed tables (twice the tables' size) are kept for the items' gradient alone
+            xp, wp = (base + at['x_pack'], base + at['w_pack']) if need_w else (wbase + packs[0], wbase + packs[1])
+            loss = torch.empty(B, dtype=torch.float32, device=dev)
+            total = None if reduction == 'none' else torch.empty((), dtype=torch.float32, device=dev)
+            L.call('igr_softmax_loss_fwd', dt, B, V, d, x.data_ptr(), ldx, items.data_ptr(), ldw, target.data_ptr(),
+                   ignore_index, scale, int(reduction == 'mean'), xp, wp, loss.data_ptr(), base + at['lse'], _p(total),
+                   None if total is None else base + at['count'], base + at['o'] if need_x else None, wbase, wsb,
+                   _stream_of(dev))
         if need_x or need_w:
-            # the packed tables (twice the tables' size) are for the items' gradient alone
-            ctx.save_for_backward(items, target, *(packs if need_w else (None, None)), lse, count, o)
-            ctx.args = (dt, B, V, d, scale, ignore_index, reduction)
-        return loss if reduction == 'none' else total
+            ctx.save_for_backward(items, target, buf)
+            ctx.args = (dt, B, V, d, ldw, scale, ignore_index, reduction, at, bwd_ws)
+        return loss if total is None else total
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        items, target, x_pack, w_pack, lse, count, o = ctx.saved_tensors
-        dt, B, V, d, scale, ignore_index, reduction = ctx.args
-        ws, ldw, _ = _table(items, 'softmax_loss items')
-        dev = ws.device
+        if torch.is_grad_enabled():  # create_graph=True (as once_differentiable would, 14 us cheaper)
+            raise IgrError('softmax_loss has no second derivative')
+        items, target, buf = ctx.saved_tensors
+        dt, B, V, d, ldw, scale, ignore_index, reduction, at, wsb = ctx.args
+        dev, base = items.device, buf.data_ptr()
+        part = lambda k: base + at[k] if k in at else None  # noqa: E731
         with _on(dev):
             grad = _f32(grad).contiguous()
-            dx = torch.empty(B, d, dtype=ws.dtype, device=dev) if ctx.needs_input_grad[0] else None
+            dx = torch.empty(B, d, dtype=items.dtype, device=dev) if ctx.needs_input_grad[0] else None
             dw = None
             if ctx.needs_input_grad[1]:
-                dw = (torch.empty if B else torch.zeros)(V, d, dtype=ws.dtype, device=dev)
-            wsb = L.lib().igr_softmax_loss_workspace_size(B, V, d, 1, 0)
-            L.call('igr_softmax_loss_bwd', dt, B, V, d, _p(ws), ldw, _p(target), ignore_index, scale,
-                   int(reduction == 'mean'), int(reduction == 'none'), _p(grad), _p(x_pack), _p(w_pack), _p(lse),
-                   _p(count), _p(o), _p(dx), _p(dw), _p(_buffer(wsb, dev)), wsb, _stream_of(dev))
+                dw = (torch.empty if B else torch.zeros)(V, d, dtype=items.dtype, device=dev)
+            ws = _buffer(wsb, dev)
+            L.call('igr_softmax_loss_bwd', dt, B, V, d, items.data_ptr(), ldw, target.data_ptr(), ignore_index, scale,
+                   int(reduction == 'mean'), int(reduction == 'none'), grad.data_ptr(), part('x_pack'), part('w_pack'),
+                   part('lse'), part('count'), part('o'), _p(dx), _p(dw), ws.data_ptr(), wsb, _stream_of(dev))
         return dx, dw, None, None, None, None
 
 

@@ -355,6 +355,26 @@ def test_table_past_32_bits():
     assert dw[:-16].abs().max() < 1e-9 and (dx[:, 1:].double() - p.matmul(W)[:, 1:] / B).abs().max() < 1e-6
 
 
+def test_second_derivatives_are_refused():
+    x, w, t = tables(20, 30, 16, torch.float32, seed=17)
+    x.requires_grad_()
+    loss = ops.softmax_loss(x, w, t)
+    with pytest.raises(IgrError, match='second derivative'):
+        torch.autograd.grad(loss, x, create_graph=True)
+
+
+def test_backward_twice_gives_the_same_bits_in_new_tensors():
+    x, w, t = tables(70, 90, 24, torch.float32, seed=18)
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.softmax_loss(x, w, t)
+    a = torch.autograd.grad(loss, (x, w), retain_graph=True)
+    kept = [g.clone() for g in a]
+    b = torch.autograd.grad(loss, (x, w), torch.tensor(1.0, device=DEV))
+    for g, k, h in zip(a, kept, b):
+        assert torch.equal(g, k) and torch.equal(g, h) and g.data_ptr() != h.data_ptr()
+
+
 def test_refusals_on_the_device():
     x, w, t = tables(4, 6, 8, torch.float32)
     with pytest.raises(IgrError, match='share'):
