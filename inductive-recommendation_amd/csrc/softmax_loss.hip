@@ -422,31 +422,36 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
 }
 
 // The loss's sum or mean over the rows that are not ignored, and their number.
-__global__ __launch_bounds__(kThreads) void softmax_reduce(int64_t B, const float *loss, const int64_t *target,
-                                                           int64_t ignore, int32_t mean, float *total,
-                                                           float *count) {
-    __shared__ double ss[kThreads];
-    __shared__ int64_t sn[kThreads];
+constexpr int kReduceThreads = 1024;
+__global__ __launch_bounds__(kReduceThreads) void softmax_reduce(int64_t B, const float *loss, const int64_t *target,
+                                                                 int64_t ignore, int32_t mean, float *total,
+                                                                 float *count) {
+    __shared__ double ss[kReduceThreads / 64];
+    __shared__ int64_t sn[kReduceThreads / 64];
     const int t = threadIdx.x;
     double s = 0.;
     int64_t n = 0;
-    for (int64_t b = t; b < B; b += kThreads) {
+    for (int64_t b = t; b < B; b += kReduceThreads) {
         s += loss[b];
         n += target[b] != ignore;
     }
-    ss[t] = s;
-    sn[t] = n;
-    __syncthreads();
-    for (int w = kThreads / 2; w; w >>= 1) {
-        if (t < w) {
-            ss[t] += ss[t + w];
-            sn[t] += sn[t + w];
-        }
-        __syncthreads();
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        n += __shfl_xor((long long)n, o, 64);
     }
+    if ((t & 63) == 0) {
+        ss[t >> 6] = s;
+        sn[t >> 6] = n;
+    }
+    __syncthreads();
     if (t == 0) {
-        *total = (float)(mean ? ss[0] / (double)(sn[0] > 0 ? sn[0] : 1) : ss[0]);
-        *count = (float)sn[0];
+        for (int w = 1; w < kReduceThreads / 64; ++w) {
+            s += ss[w];
+            n += sn[w];
+        }
+        *total = (float)(mean ? s / (double)(n > 0 ? n : 1) : s);
+        *count = (float)n;
     }
 }
 
@@ -502,9 +507,17 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     if (t == 0) cm = -250;
     __syncthreads();
     int c_all = -250;
-    for (int64_t b = t; b < a.B; b += kThreads) {
-        const float c = fabsf(row_coef(a, b, a.target[b]));
-        if (c > 0.f) c_all = max(c_all, block_exponent(c) + (SCALED ? a.x.exps[b / kRB] : 0));
+    if (a.per_row) {
+        for (int64_t b = t; b < a.B; b += kThreads) {
+            const float c = fabsf(row_coef(a, b, a.target[b]));
+            if (c > 0.f) c_all = max(c_all, block_exponent(c) + (SCALED ? a.x.exps[b / kRB] : 0));
+        }
+    } else {  // one coefficient; blocks of nothing but ignored rows are packed as zeros and do not count
+        const float c = a.grad[0] * a.scale / (a.mean ? fmaxf(*a.count, 1.f) : 1.f);
+        const int e = block_exponent(fabsf(c));
+        if (!SCALED) c_all = e;
+        else
+            for (int64_t k = t; k < blocks_of(a.B); k += kThreads) c_all = max(c_all, e + a.x.exps[k]);
     }
     atomicMax(&cm, c_all);  // in LDS; a maximum does not depend on the order
     __syncthreads();
@@ -880,7 +893,7 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
             if (rc) return rc;
         }
         if (total)
-            hipLaunchKernelGGL(softmax_reduce, dim3(1), dim3(kThreads), 0, st, b, loss, target, ignore_index, mean, total,
+            hipLaunchKernelGGL(softmax_reduce, dim3(1), dim3(kReduceThreads), 0, st, b, loss, target, ignore_index, mean, total,
                                count);
         return launch_status(fn);
     });
