@@ -27,9 +27,9 @@
 //
 // Bound by the matrix cores and, beside them, the softmax's own arithmetic (an exponential, a
 // subtraction and two conversions a weight).  B = 2048, d = 64, fp32: one million items take 1.55 ms
-// forward and 1.3 ms backward, 1.1 to 1.25 PFLOP/s of fp16 products (a large library product: 1.55);
-// 40,981 items 80 and 88 us.  32 NB rows a wave are what 256 registers hold: with NB = 1 each
-// fragment read from LDS serves half the products and the million takes half as long again.
+// forward and 1.3 ms backward, 1.1 to 1.25 PFLOP/s of fp16 products.  On operands that are not constant
+// MFMAs alone sustain 1.56 here (2.3 on constants: the clock falls with what they switch), a large
+// library product 1.55.  40,981 items take 80 and 87 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -153,6 +153,25 @@ __device__ __forceinline__ void load_frags(const u32x4_t *base, int f, int lane,
         fr.p[n] = __builtin_bit_cast(typename P::frag, base[(f * P::NS + n) * 64 + lane]);
 }
 
+// acc[n] += a streamed block's rows times the NB blocks of rows held in registers, over the width.  Four
+// steps' fragments are read from LDS before the first of their MFMAs: read one by one right before its
+// use, as the compiler orders them, each waits for LDS (1500 x 50,021 x 200 bf16: forward
+// 183 us, like this 170; at d = 64 the other workgroup covers most of it).
+template <class P, int KS, int NB, class B>
+__device__ __forceinline__ void logits(const u32x4_t *lds, int lane, const B &held, f32x16_t (&acc)[NB]) {
+    constexpr int G = KS < 4 ? KS : 4;
+#pragma unroll
+    for (int s0 = 0; s0 < KS; s0 += G) {
+        Frags<P> f[G];
+#pragma unroll
+        for (int s = 0; s < G; ++s) load_frags<P>(lds, s0 + s, lane, f[s]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < G; ++s)
+            mfma_row<P, NB>(f[s], [&](int n) -> const Frags<P> & { return held(n, s0 + s); }, acc);
+    }
+}
+
 struct FwdArgs {
     int64_t B, V, nbt, splits, per;  // batch tiles, catalogue splits, item blocks per split
     Packed x, w;
@@ -235,12 +254,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            Frags<P> wf;
-            load_frags<P>(w, s, lane, wf);
-            mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return xf[n][s]; }, acc);
-        }
+        logits<P, KS, NB>(w, lane, [&](int n, int s) -> const Frags<P> & { return xf[n][s]; }, acc);
         const int v0 = (int)(k * kRB);
         const int nv = a.V - k * kRB < kRB ? (int)(a.V - k * kRB) : kRB;  // items of this block
         Frags<P> pf[NB][2];
@@ -635,12 +649,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            Frags<P> xf;
-            load_frags<P>(x, s, lane, xf);
-            mfma_row<P, NB>(xf, [&](int n) -> const Frags<P> & { return wf[n][s]; }, acc);
-        }
+        logits<P, KS, NB>(x, lane, [&](int n, int s) -> const Frags<P> & { return wf[n][s]; }, acc);
         // lane: item v0 + col; register i: batch row 8 (i/4) + 4 h + i%4 of the block
         const int tcol = __builtin_bit_cast(int, info[2][col]);
         Frags<P> pf[NB][2];
