@@ -1395,10 +1395,11 @@ def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):
         return t, max(t.stride(0), k)
     a, lda = rows(a)
     b, ldb = rows(b)
+    a_scale, b_scale = a_scale.contiguous(), b_scale.contiguous()
     with _on(a.device):
         c = torch.empty(m, n, dtype=out_dtype, device=a.device)
-        L.call('igr_gemm_int8', m, n, k, _p(a), lda, _p(a_scale.contiguous()), _p(b), ldb, _p(b_scale.contiguous()),
-               _DTYPES[out_dtype], _p(c), n, _stream_of(a.device))
+        L.call('igr_gemm_int8', m, n, k, _p(a), lda, _p(a_scale), _p(b), ldb, _p(b_scale), _DTYPES[out_dtype], _p(c),
+               n, _stream_of(a.device))
     return c
 
 

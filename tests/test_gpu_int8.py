@@ -111,6 +111,13 @@ def test_product_of_strided_and_unaligned_tables(k, pad):
     assert torch.equal(y, ops.gemm_int8(a, sa, t, sb))
 
 
+def test_both_scales_strided():
+    """Each side's packed copy of its scales outlives the launch, not only the other copy's allocation."""
+    a, sa, b, sb = tables(40, 50, 64, seed=3)
+    wide_a, wide_b = sa.repeat_interleave(2), sb.repeat_interleave(3)
+    assert torch.equal(ops.gemm_int8(a, wide_a[::2], b, wide_b[::3]), check_product(a, sa, b, sb, torch.float32))
+
+
 def test_extreme_sums_and_scales():
     a = torch.full((40, 131071), -128, dtype=torch.int8, device=DEV)  # the largest sum that is allowed
     one = torch.ones(40, device=DEV)
