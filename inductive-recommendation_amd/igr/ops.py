@@ -1350,6 +1350,8 @@ def softmax_loss(x, items, target, scale=1.0, ignore_index=-100, reduction='mean
         raise IgrError('softmax_loss: no items')
     if not (scale > 0 and math.isfinite(scale)):
         raise IgrError(f'softmax_loss: scale must be positive and finite, got {scale}')
+    if not torch.is_grad_enabled():  # needs_input_grad does not know: no weighted sums of items for a loss alone
+        x, items = x.detach(), items.detach()
     return SoftmaxLoss.apply(x, items, target.to(torch.int64).contiguous(), float(scale), int(ignore_index), reduction)
 
 

@@ -275,6 +275,18 @@ def test_one_sided_gradients_and_no_grad():
     assert not l3.requires_grad and torch.equal(l1, l3) and torch.equal(l2, l3)
 
 
+def test_no_grad_keeps_nothing_for_a_backward(monkeypatch):
+    x, w, t = tables(90, 210, 40, torch.float32, seed=13)
+    x.requires_grad_()
+    w.requires_grad_()
+    asked = []
+    layout = ops._softmax_layout
+    monkeypatch.setattr(ops, '_softmax_layout', lambda *a: asked.append(a[4:]) or layout(*a))
+    with torch.no_grad():
+        quiet = ops.softmax_loss(x, w, t)
+    assert torch.equal(quiet, ops.softmax_loss(x, w, t)) and asked == [(False, False), (True, True)]
+
+
 def test_same_bits_again_and_on_another_stream():
     x, w, t = tables(513, 3333, 64, torch.float32, seed=14)
     a = check(x, w, t)
