@@ -553,7 +553,7 @@ int igr_layer_tail_bwd_f32(int64_t n, int32_t d, const float *gn, int64_t ldgn, 
  *                      sum_v softmax_bv items_v without the target for dx; NULL if dx will not be asked for
  * The workspace holds igr_softmax_loss_workspace_size(b, v, d, 0, o != NULL) bytes.  fp32
  * products run on the 16-bit matrix cores in three parts with fp32's accuracy; half types
- * multiply as they are and round the softmax weights once.  Fixed summation order. */
+ * multiply as they are, with softmax weights of twice their digits.  Fixed summation order. */
 int64_t igr_softmax_loss_pack_size(int64_t rows, int32_t d, int32_t dtype);
 int64_t igr_softmax_loss_workspace_size(int64_t b, int64_t v, int32_t d, int32_t backward, int32_t with_o);
 int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *x, int64_t ldx,

@@ -172,6 +172,26 @@ __device__ __forceinline__ void logits(const u32x4_t *lds, int lane, const B &he
     }
 }
 
+// A tile's weights as operands of the product with the table's rows.  fp32's are pairs of halves already;
+// half types' become pairs too, what the first rounding left as the second operand: rounded once, a weight
+// is off by half a step (2^-8 of it for bf16), and a sum of few large weights by as much.  1500 x 50,021 x
+// 200 in bf16: rounded once, the items' gradient, whose target's term often is nearly all there is, is off by
+// 2.8e-3 of its norm, as pairs by 1.7e-3, the result's own rounding; x's gradient differs from one of 32-bit
+// weights by 2.6e-4 and 9e-5 of its norm.  The second product costs the forward 160 -> 195 us.
+template <class P, int NR>
+__device__ __forceinline__ void split_weights(float (&p)[16], Frags<P> (&w)[2], Frags<P> (&rest)[NR]) {
+    float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
+    float (&ph)[8] = reinterpret_cast<float (&)[8]>(p[8]);
+    split8(pl, w[0]);
+    split8(ph, w[1]);
+    if constexpr (P::NS == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] -= (float)w[i >> 3].p[0][i & 7];
+        split8(pl, rest[0]);
+        split8(ph, rest[1]);
+    }
+}
+
 struct FwdArgs {
     int64_t B, V, nbt, splits, per;  // batch tiles, catalogue splits, item blocks per split
     Packed x, w;
@@ -258,6 +278,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
         const int v0 = (int)(k * kRB);
         const int nv = a.V - k * kRB < kRB ? (int)(a.V - k * kRB) : kRB;  // items of this block
         Frags<P> pf[NB][2];
+        Frags<P> rest[NB][P::NS == 1 ? 2 : 1];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             // lane: batch row `col` of block n; register i: item 8 (i/4) + 4 h + i%4
@@ -309,12 +330,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
                 s1 += p[i + 1];
             }
             z[n] = fmaf(s0 + s1, pow2f(-sh), z[n]);
-            if constexpr (WITH_O) {
-                float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
-                float (&ph)[8] = reinterpret_cast<float (&)[8]>(p[8]);
-                split8(pl, pf[n][0]);
-                split8(ph, pf[n][1]);
-            }
+            if constexpr (WITH_O) split_weights<P>(p, pf[n], rest[n]);
         }
         if constexpr (WITH_O) {
 #pragma unroll
@@ -323,6 +339,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
                 load_frags<P>(w, KS + f, lane, wf);
                 f32x16_t (&of)[NB] = o[f >> 1];
                 mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
+                if constexpr (P::NS == 1) mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return rest[n][f & 1]; }, of);
             }
         }
         copies_done();
@@ -677,19 +694,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
                     if (__builtin_bit_cast(int, info[2][r]) == v0[n] + col) p[i] = -info[1][r];
                 }
             }
-            float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
-            float (&ph)[8] = reinterpret_cast<float (&)[8]>(p[8]);
-            split8(pl, pf[n][0]);
-            split8(ph, pf[n][1]);
-            if constexpr (P::NS == 1) {
-                // Half types: the weight as a pair of them, what the first rounding left as the second.  A
-                // target's term often is nearly all of its item's gradient, and rounded once it took the
-                // gradient's error from 1.7e-3 of its norm, the result's own rounding, to 2.8e-3 (bf16).
-#pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] -= (float)pf[n][i >> 3].p[0][i & 7];
-                split8(pl, rest[n][0]);
-                split8(ph, rest[n][1]);
-            }
+            split_weights<P>(p, pf[n], rest[n]);
         }
 #pragma unroll
         for (int f = 0; f < 2 * DB; ++f) {
