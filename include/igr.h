@@ -552,8 +552,12 @@ int igr_layer_tail_bwd_f32(int64_t n, int32_t d, const float *gn, int64_t ldgn, 
  *   o                  [b, 32 / 64 / 128 / 256 - the next that holds d] rows of
  *                      sum_v softmax_bv items_v without the target for dx; NULL if dx will not be asked for
  * The workspace holds igr_softmax_loss_workspace_size(b, v, d, 0, o != NULL) bytes.  fp32
- * products run on the 16-bit matrix cores in three parts with fp32's accuracy; half types
- * multiply as they are, with softmax weights of twice their digits.  Fixed summation order. */
+ * products run on the 16-bit matrix cores in three parts with fp32's accuracy, each row's entries
+ * to 2^-23 of its largest whatever the other rows are; a term of a gradient is held to 2^-37 of the
+ * largest (of the row's terms in dx; in dw of the batch's c_b x_b, c_b the incoming gradients).
+ * Infinite or NaN entries of fp32 tables make what they enter NaN (an item is masked by finite
+ * entries, down to the type's lowest).  Half types multiply as they are, with softmax weights of
+ * twice their digits.  Fixed summation order. */
 int64_t igr_softmax_loss_pack_size(int64_t rows, int32_t d, int32_t dtype);
 int64_t igr_softmax_loss_workspace_size(int64_t b, int64_t v, int32_t d, int32_t backward, int32_t with_o);
 int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t d, const void *x, int64_t ldx,

@@ -2,8 +2,8 @@
 // multiply fp32 tables on the 16-bit matrix cores.
 //
 // An fp32 value is held as a pair of halves: x 2^s = hi + lo, hi = fp16(x 2^s) and
-// lo = fp16(x 2^s - hi), with s a power of two shared by a block, so that the block's largest
-// entry lies in [2^14, 2^15).  hi + lo carries 23 bits of x, down to 2^-39 of the block's
+// lo = fp16(x 2^s - hi), with s a power of two shared by a row (or by rows of like size), so that the
+// largest entry lies in [2^14, 2^15).  hi + lo carries 23 bits of x, down to 2^-39 of that
 // largest entry (fp16's smallest subnormal is 2^-24).  A product is three MFMAs,
 // hi hi + hi lo + lo hi, summed in fp32; the lo lo term, 2^-22 of the product, is left out.
 // That is fp32's accuracy over sums of 64 and more terms at a third of the fp16 rate: 518 TFLOP/s

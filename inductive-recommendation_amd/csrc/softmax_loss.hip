@@ -53,15 +53,35 @@ __host__ __device__ constexpr int block_halves(int dp) { return 2 * P::NS * kRB 
 inline int64_t block_bytes(int32_t dtype, int dp) { return (dtype == kF32 ? 2 : 1) * 2ll * kRB * dp * 2; }
 inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
 
-// A packed table: its blocks, then one exponent per block.
+// A packed table: its blocks, then fp32's exponents: a row's entries are held times 2^(14 - its own).  A block
+// whose rows are within 2^kNarrow of each other has one exponent for all of them (its largest row's), and
+// the kernels their short path; the digits of a row 2^8 below it still reach 2^-31 of its largest entry.  In
+// the others each row has its own, however large its neighbours are (an item masked by
+// an entry of -1e9 or the type's lowest value).
 struct Packed {
     const u32x4_t *blocks;
-    const int32_t *exps;
+    const int32_t *exps;      // per block: its largest row's, plus kWide where rows have their own
+    const int8_t *row_exps;   // per row, padded to whole blocks
 };
+constexpr int kNarrow = 8, kWide = 1024, kZeros = -101;  // kZeros: a block of zeros
 inline Packed packed_view(const void *p, int64_t rows, int32_t dtype, int dp) {
-    const char *c = static_cast<const char *>(p);
-    return Packed{reinterpret_cast<const u32x4_t *>(c),
-                  reinterpret_cast<const int32_t *>(c + blocks_of(rows) * block_bytes(dtype, dp))};
+    const char *c = static_cast<const char *>(p) + blocks_of(rows) * block_bytes(dtype, dp);
+    return Packed{static_cast<const u32x4_t *>(p), reinterpret_cast<const int32_t *>(c),
+                  reinterpret_cast<const int8_t *>(c + blocks_of(rows) * sizeof(int32_t))};
+}
+__host__ __device__ inline int largest_exp(int e) { return e >= kWide / 2 ? e - kWide : e; }
+__host__ __device__ inline bool is_wide(int e) { return e >= kWide / 2; }
+// f(i, exponent of register i's row) for the 16 rows that a lane of half h holds of block k's product.  Read where
+// they are used (volatile: kept from there to there they cost the short path its registers).
+template <class F>
+__device__ __forceinline__ void each_exp(const int8_t *row_exps, int64_t k, int h, F &&f) {
+    const volatile int32_t *p = reinterpret_cast<const volatile int32_t *>(row_exps + k * kRB) + h;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int32_t v = p[2 * g];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f(4 * g + i, (int)(int8_t)(v >> (8 * i)));
+    }
 }
 
 struct PackArgs {
@@ -69,6 +89,7 @@ struct PackArgs {
     const void *src;
     u32x4_t *blocks;
     int32_t *exps;
+    int8_t *row_exps;
     const int64_t *target;  // rows whose target is `ignore` are packed as zeros; NULL: none
     int64_t ignore;
 };
@@ -78,19 +99,28 @@ struct PackArgs {
 template <class P, int DP>
 __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, int64_t n0, int32_t d, int32_t vec) {
     __shared__ float tile[kRB][DP + 1];
-    __shared__ float wmax[kThreads / 64];
+    __shared__ uint32_t rmax[kRB];  // bits of the rows' largest finite magnitudes
     const int64_t blk = blockIdx.x < n0 ? blockIdx.x : blockIdx.x - n0;
     const PackArgs a = blockIdx.x < n0 ? a0 : a1;
     const typename P::elem *src = static_cast<const typename P::elem *>(a.src);
     const int64_t r0 = blk * kRB;
     const int t = threadIdx.x;
     constexpr int VE = 16 / sizeof(typename P::elem);
-    float amax = 0.f;
-    auto put = [&](int r, int c, float v) {
-        tile[r][c] = v;
-        const float m = fabsf(v);
-        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);  // finite entries set the scale
+    if constexpr (P::kScaled) {
+        if (t < kRB) rmax[t] = 0;
+        __syncthreads();
+    }
+    // row r's magnitudes, G neighbouring lanes of it at a time
+    auto note = [&](int r, float amax, auto lanes) {
+        constexpr int G = decltype(lanes)::value < 64 ? decltype(lanes)::value : 64;
+        if constexpr (P::kScaled) {
+#pragma unroll
+            for (int o = G / 2; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
+            // in LDS; a maximum does not depend on the order
+            if (t % G == 0) atomicMax(&rmax[r], __builtin_bit_cast(uint32_t, amax));
+        }
     };
+    auto finite = [](float v) { return fabsf(v) <= 3.402823466e38f ? fabsf(v) : 0.f; };  // finite entries set the scale
     if (vec) {  // rows of whole 16-byte groups
         for (int i = t; i < kRB * DP / VE; i += kThreads) {
             const int r = i / (DP / VE), c = (i % (DP / VE)) * VE;
@@ -100,8 +130,13 @@ __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, 
                 raw = *reinterpret_cast<const u32x4_t *>(src + gr * a.ld + c);
             typename P::elem e[VE];
             __builtin_memcpy(e, &raw, 16);
+            float amax = 0.f;
 #pragma unroll
-            for (int j = 0; j < VE; ++j) put(r, c + j, (float)e[j]);
+            for (int j = 0; j < VE; ++j) {
+                tile[r][c + j] = (float)e[j];
+                amax = fmaxf(amax, finite((float)e[j]));
+            }
+            note(r, amax, std::integral_constant<int, DP / VE>());
         }
     } else {
         for (int i = t; i < kRB * DP; i += kThreads) {
@@ -109,25 +144,32 @@ __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, 
             const int64_t gr = r0 + r;
             float v = 0.f;
             if (gr < a.rows && c < d && !(a.target && a.target[gr] == a.ignore)) v = (float)src[gr * a.ld + c];
-            put(r, c, v);
+            tile[r][c] = v;
+            note(r, finite(v), std::integral_constant<int, DP>());
         }
     }
-    int e = 0;
-    float s = 1.f;
-    if constexpr (P::kScaled) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o, 64));
-        if ((t & 63) == 0) wmax[t >> 6] = amax;
-    }
     __syncthreads();
+    const int lane = t & 63, col = lane & 31, h = lane >> 5;
+    int e = 0;              // the exponent of row `col`
+    float s = 1.f;          // and its scale
+    bool wide = false;
     if constexpr (P::kScaled) {
-        e = block_exponent(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])));
+        const float amax = __builtin_bit_cast(float, rmax[col]);
+        e = block_exponent(amax);
+        int most = e, least = amax > 0.f ? e : 127;  // rows of zeros are as narrow as any
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            most = max(most, __shfl_xor(most, o, 64));
+            least = min(least, __shfl_xor(least, o, 64));
+        }
+        wide = __builtin_amdgcn_readfirstlane(most - least) > kNarrow;
+        if (!wide || amax == 0.f) e = most;
         s = pow2f(P::kOff - e);
+        if (t < kRB) a.row_exps[r0 + t] = (int8_t)e;
+        if (t == 0) a.exps[blk] = least == 127 && most == -100 ? kZeros : most + (wide ? kWide : 0);
     }
-    if (t == 0) a.exps[blk] = e;
     u32x4_t *out = a.blocks + blk * (block_halves<P>(DP) / 8);
     constexpr int KS = DP / 16, DB = DP / 32;
-    const int lane = t & 63, col = lane & 31, h = lane >> 5;
     for (int f = t >> 6; f < 2 * KS; f += kThreads / 64) {
         float v[8];
         if (f < KS) {
@@ -136,7 +178,10 @@ __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, 
         } else {
             const int g = f - KS, db = g >> 1, st = g & 1;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = tile[16 * st + 8 * (i >> 2) + 4 * h + (i & 3)][db * 32 + col] * s;
+            for (int i = 0; i < 8; ++i) {
+                const int r = 16 * st + 8 * (i >> 2) + 4 * h + (i & 3);
+                v[i] = tile[r][db * 32 + col] * (wide ? __shfl(s, r, 64) : s);
+            }
         }
         Frags<P> fr;
         split8(v, fr);
@@ -198,7 +243,7 @@ struct FwdArgs {
     const int64_t *target;
     float scale2;  // scale log2(e)
     float *pm, *pz, *pt, *po;  // partials: [splits][B] max (log2), sum without the target, its logit; [splits][B][DP]
-    int32_t *pc;               // [splits] exponent of po
+    int32_t *pd;               // [splits][B] exponent of po
 };
 
 // WITH_O = false: the loss alone (no product with the T part, which is then not copied either).
@@ -209,7 +254,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
     constexpr int TILE = block_halves<P>(DP) / 8 / (WITH_O ? 1 : 2);  // u32x4_t of a streamed block
     constexpr int BLK = block_halves<P>(DP) / 8;
     __shared__ u32x4_t lds0[TILE], lds1[TILE];
-    __shared__ int32_t cmax_s;
+    __shared__ int32_t most_s, least_s;
     // workgroups of one split sit on one XCD (blockIdx % 8), next to each other in time: the
     // split's item blocks come from that XCD's L2 for all batch tiles but the first
     const int64_t id = blockIdx.x, xcd = id & 7, j = id >> 3;
@@ -220,169 +265,219 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
     const int64_t k0 = split * a.per, k1 = k0 + a.per < nblk ? k0 + a.per : nblk;
     const int64_t nxb = blocks_of(a.B);
 
-    // exponent that the weights of the split's blocks are made for: the largest of the split's blocks
+    // The exponents of the split's blocks.  Where they are within 2^kNarrow of each other, as a trained table's are,
+    // the weights are made for the largest, C; else for what weighs most so far, row by row of the batch
+    // (a large item that weighs nothing must not push the others' weights out of the halves' range).  With an
+    // item in 1000 masked by -1e9, 2048 x a million x 64 takes 3.0 ms forward instead of 1.55.
     int C = 0;
+    bool even = true;
     if constexpr (P::kScaled) {
-        if (t == 0) cmax_s = -127;
+        if (t == 0) most_s = -127, least_s = 127;
         __syncthreads();
-        int c = -127;
-        for (int64_t k = k0 + t; k < k1; k += kThreads) c = max(c, a.w.exps[k]);
-        atomicMax(&cmax_s, c);  // in LDS; a maximum does not depend on the order
-        __syncthreads();
-        C = __builtin_amdgcn_readfirstlane(cmax_s);
-    }
-
-    // this wave's batch blocks
-    Frags<P> xf[NB][KS];
-    float c_x[NB], m[NB], z[NB], tl[NB];
-    int tgt[NB];
-    bool live[NB];
-    f32x16_t o[WITH_O ? DB : 1][NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int64_t xb = (bt * 4 + wave) * NB + n;
-        live[n] = xb < nxb;
-        const int64_t xs = live[n] ? xb : 0;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) load_frags<P>(a.x.blocks + xs * BLK, k, lane, xf[n][k]);
-        c_x[n] = a.scale2 * (P::kScaled ? pow2f(a.x.exps[xs] - P::kOff) : 1.f);
-        m[n] = -INFINITY;
-        z[n] = 0.f;
-        tl[n] = 0.f;
-        const int64_t b = xs * kRB + col;
-        const int64_t tt = live[n] && b < a.B ? a.target[b] : -1;
-        tgt[n] = tt >= 0 && tt < a.V ? (int)tt : -1;
-#pragma unroll
-        for (int q = 0; q < (WITH_O ? DB : 1); ++q)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[q][n][i] = 0.f;
-    }
-
-    // w: the block in LDS that is used; next: the buffer that the following block is copied to meanwhile.
-    // (Two arrays by name, and the loop in pairs: so the compiler sees that reading one need not wait for
-    // the copy into the other.)
-    int ew_next = P::kScaled ? a.w.exps[k0] : 0;  // loaded a block ahead, before that block's copy is begun
-    auto step = [&](int64_t k, const u32x4_t *__restrict__ w, u32x4_t *__restrict__ next) {
-        const int ew = P::kScaled ? __builtin_amdgcn_readfirstlane(ew_next) : 0;
-        if (k + 1 < k1) {
-            if (P::kScaled) ew_next = a.w.exps[k + 1];
-            copy_to_lds<TILE>(a.w.blocks + (k + 1) * BLK, next, t);
+        int most = -127, least = 127;
+        for (int64_t k = k0 + t; k < k1; k += kThreads) {
+            const int e = a.w.exps[k];
+            most = max(most, largest_exp(e));
+            if (e != kZeros) least = min(least, is_wide(e) ? -1000 : e);
         }
-        const float c_w = P::kScaled ? pow2f(ew - P::kOff) : 1.f;
-        f32x16_t acc[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
-        logits<P, KS, NB>(w, lane, [&](int n, int s) -> const Frags<P> & { return xf[n][s]; }, acc);
-        const int v0 = (int)(k * kRB);
-        const int nv = a.V - k * kRB < kRB ? (int)(a.V - k * kRB) : kRB;  // items of this block
-        Frags<P> pf[NB][2];
-        Frags<P> rest[NB][P::NS == 1 ? 2 : 1];
+        const int64_t xb = bt * 4 * NB + t;  // and no batch row of the workgroup has its own
+        if (t < 4 * NB && xb < nxb && is_wide(a.x.exps[xb])) least = -1000;
+        atomicMax(&most_s, most);  // in LDS; these do not depend on the order
+        atomicMin(&least_s, least);
+        __syncthreads();
+        C = __builtin_amdgcn_readfirstlane(most_s);
+        even = C - __builtin_amdgcn_readfirstlane(least_s) <= kNarrow;
+    }
+
+    // EVEN: one exponent a block; else every row has its own.  The two share neither variables nor, for the differing
+    // asm lines, loads: with one loop for both, or shared loads before two, the first reloaded spilled
+    // registers in each step (2048 x a million x 64: 2390 and 1882 us, like this 1546).
+    auto body = [&](auto kind) __attribute__((always_inline)) {
+        constexpr bool EVEN = decltype(kind)::value;
+        if constexpr (EVEN) asm volatile("; one exponent a block");
+        else asm volatile("; one exponent a row");
+        // this wave's batch blocks
+        Frags<P> xf[NB][KS];
+        // top: the largest log2 of a weight times its row's power of two so far
+        float c_x[NB], m[NB], top[NB], z[NB], tl[NB];
+        int tgt[NB];
+        bool live[NB];
+        f32x16_t o[WITH_O ? DB : 1][NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
-            // lane: batch row `col` of block n; register i: item 8 (i/4) + 4 h + i%4
-            // (c of two tables of zeros would round to 0, and 0 times infinity is none)
-            const float c = fmaxf(c_x[n] * c_w, 1.17549435e-38f);
-            if (__any((unsigned)(tgt[n] - v0) < 32u)) {  // some row's target is here: its logit apart from the others
+            const int64_t xb = (bt * 4 + wave) * NB + n;
+            live[n] = xb < nxb;
+            const int64_t xs = live[n] ? xb : 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (tgt[n] - v0 == 8 * (i >> 2) + 4 * h + (i & 3)) {
-                        tl[n] = acc[n][i] * c;
-                        acc[n][i] = -INFINITY;
+            for (int k = 0; k < KS; ++k) load_frags<P>(a.x.blocks + xs * BLK, k, lane, xf[n][k]);
+            if constexpr (!P::kScaled) c_x[n] = a.scale2;
+            else c_x[n] = a.scale2 * pow2f((EVEN ? largest_exp(a.x.exps[xs]) : a.x.row_exps[xs * kRB + col]) - P::kOff);
+            m[n] = top[n] = -INFINITY;
+            z[n] = 0.f;
+            tl[n] = 0.f;
+            const int64_t b = xs * kRB + col;
+            const int64_t tt = live[n] && b < a.B ? a.target[b] : -1;
+            tgt[n] = tt >= 0 && tt < a.V ? (int)tt : -1;
+#pragma unroll
+            for (int q = 0; q < (WITH_O ? DB : 1); ++q)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[q][n][i] = 0.f;
+        }
+
+        // w: the block in LDS that is used; next: the buffer that the following block is copied to meanwhile.
+        // (Two arrays by name, and the loop in pairs: so the compiler sees that reading one need not wait for
+        // the copy into the other.)
+        // o is held times 2^(14 - C or down) and its rows' 2^14: the largest product's weight is 2^14 in the halves' range
+        auto down_of = [](float top, float m) { return m > -INFINITY ? (int)ceilf(top - m) : 0; };
+        int ew_next = P::kScaled ? a.w.exps[k0] : 0;  // loaded a block ahead, before that block's copy is begun
+        auto step = [&](int64_t k, const u32x4_t *__restrict__ w, u32x4_t *__restrict__ next) __attribute__((always_inline)) {
+            const int ew = P::kScaled ? largest_exp(__builtin_amdgcn_readfirstlane(ew_next)) : 0;
+            if (k + 1 < k1) {
+                if (P::kScaled) ew_next = a.w.exps[k + 1];
+                copy_to_lds<TILE>(a.w.blocks + (k + 1) * BLK, next, t);
+            }
+            const float c_w = P::kScaled ? pow2f(ew - P::kOff) : 1.f;
+            f32x16_t acc[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
+            logits<P, KS, NB>(w, lane, [&](int n, int s) -> const Frags<P> & { return xf[n][s]; }, acc);
+            if constexpr (!EVEN)
+                each_exp(a.w.row_exps, k, h, [&](int i, int e) {
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) acc[n][i] = ldexpf(acc[n][i], e - ew);
+                });
+            const int v0 = (int)(k * kRB);
+            const int nv = a.V - k * kRB < kRB ? (int)(a.V - k * kRB) : kRB;  // items of this block
+            Frags<P> pf[NB][2];
+            Frags<P> rest[NB][P::NS == 1 ? 2 : 1];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                // lane: batch row `col` of block n; register i: item 8 (i/4) + 4 h + i%4
+                // (c of two tables of zeros would round to 0, and 0 times infinity is none)
+                const float c = fmaxf(c_x[n] * c_w, 1.17549435e-38f);
+                if (__any((unsigned)(tgt[n] - v0) < 32u)) {  // some row's target is here: its logit apart from the others
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (tgt[n] - v0 == 8 * (i >> 2) + 4 * h + (i & 3)) {
+                            tl[n] = acc[n][i] * c;
+                            acc[n][i] = -INFINITY;
+                        }
+                }
+                if (nv < kRB) {  // the catalogue's last block: its padding takes no part
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (8 * (i >> 2) + 4 * h + (i & 3) >= nv) acc[n][i] = -INFINITY;
+                }
+                float mx = acc[n][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[n][i]);
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+                float mt = -INFINITY;  // the largest log2 of the block's weights times their rows' powers of two
+                if constexpr (!EVEN) {
+                    each_exp(a.w.row_exps, k, h, [&](int i, int e) { mt = fmaxf(mt, fmaf(acc[n][i], c, (float)e)); });
+                    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+                }
+                if (__any(mx > m[n] || (!EVEN && mt > top[n]))) {  // rare after the first blocks
+                    const float mn = fmaxf(m[n], mx);
+                    const float less = m[n] == mn ? 0.f : m[n] - mn;  // (both may be -infinity)
+                    const float f = __builtin_amdgcn_exp2f(less);
+                    z[n] *= f;
+                    float fo = f;
+                    if constexpr (!EVEN) {
+                        const float tn = fmaxf(top[n], mt);
+                        fo = __builtin_amdgcn_exp2f(less + (float)(down_of(top[n], m[n]) - down_of(tn, mn)));
+                        top[n] = tn;
                     }
-            }
-            if (nv < kRB) {  // the catalogue's last block: its padding takes no part
+                    m[n] = mn;
+                    if constexpr (WITH_O) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (8 * (i >> 2) + 4 * h + (i & 3) >= nv) acc[n][i] = -INFINITY;
-            }
-            float mx = acc[n][0];
+                        for (int q = 0; q < DB; ++q)
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[n][i]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-            if (__any(mx > m[n])) {  // rare after the first blocks
-                const float mn = fmaxf(m[n], mx);
-                const float f = m[n] == mn ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);  // (both may be -infinity)
-                m[n] = mn;
-                z[n] *= f;
+                            for (int i = 0; i < 16; ++i) o[q][n][i] *= fo;
+                    }
+                }
+                // weights p 2^sh: up to 2^14 in the halves' range, less where the block's rows are
+                // smaller than the split's largest.  -60 keeps the sum exact; a block that far
+                // below adds nothing to o either way.
+                // (without o the same powers, for the same sums bit for bit)
+                const int sh = EVEN ? 14 + (P::kScaled ? max(ew - C, -60) : 0) : 0;
+                // (no maximum yet: the target is the only item so far)
+                const float off = m[n] == -INFINITY ? 0.f : m[n] - (float)sh;
+                float p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    s0 += p[i];
+                    s1 += p[i + 1];
+                }
+                z[n] = fmaf(s0 + s1, pow2f(-sh), z[n]);
                 if constexpr (WITH_O) {
-#pragma unroll
-                    for (int q = 0; q < DB; ++q)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[q][n][i] *= f;
+                    if constexpr (!EVEN) {  // each weight by its own row's power, up to 2^14 again
+                        const int up = 14 - down_of(top[n], m[n]);
+                        each_exp(a.w.row_exps, k, h, [&](int i, int e) { p[i] = ldexpf(p[i], e + up); });
+                    }
+                    split_weights<P>(p, pf[n], rest[n]);
                 }
             }
-            // weights p 2^sh: up to 2^14 in the halves' range, less where the block's rows are
-            // smaller than the split's largest.  -60 keeps the sum exact; a block that far
-            // below adds nothing to o either way.
-            // (without o the same powers, for the same sums bit for bit)
-            const int sh = 14 + (P::kScaled ? max(ew - C, -60) : 0);
-            // (no maximum yet: the target is the only item so far)
-            const float off = m[n] == -INFINITY ? 0.f : m[n] - (float)sh;
-            float p[16];
+            if constexpr (WITH_O) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                s0 += p[i];
-                s1 += p[i + 1];
+                for (int f = 0; f < 2 * DB; ++f) {
+                    Frags<P> wf;
+                    load_frags<P>(w, KS + f, lane, wf);
+                    f32x16_t (&of)[NB] = o[f >> 1];
+                    mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
+                    if constexpr (P::NS == 1) mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return rest[n][f & 1]; }, of);
+                }
             }
-            z[n] = fmaf(s0 + s1, pow2f(-sh), z[n]);
-            if constexpr (WITH_O) split_weights<P>(p, pf[n], rest[n]);
-        }
-        if constexpr (WITH_O) {
-#pragma unroll
-            for (int f = 0; f < 2 * DB; ++f) {
-                Frags<P> wf;
-                load_frags<P>(w, KS + f, lane, wf);
-                f32x16_t (&of)[NB] = o[f >> 1];
-                mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
-                if constexpr (P::NS == 1) mfma_row<P, NB>(wf, [&](int n) -> const Frags<P> & { return rest[n][f & 1]; }, of);
-            }
-        }
+            copies_done();
+            __syncthreads();
+        };
+        copy_to_lds<TILE>(a.w.blocks + k0 * BLK, lds0, t);
         copies_done();
         __syncthreads();
+        for (int64_t k = k0; k < k1; k += 2) {
+            step(k, lds0, lds1);
+            if (k + 1 < k1) step(k + 1, lds1, lds0);
+        }
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const int64_t b = ((bt * 4 + wave) * NB + n) * kRB + col;
+            // the two halves of a row: same maximum, sums of different items, one target logit
+            const float zz = z[n] + __shfl_xor(z[n], 32, 64);
+            const float ot = __shfl_xor(tl[n], 32, 64);
+            const bool mine = (tgt[n] >> 2 & 1) == h;  // items 8q + 4h + 0..3 are this half's
+            if (!live[n] || b >= a.B) continue;
+            if (h == 0) {
+                a.pm[split * a.B + b] = m[n];
+                a.pz[split * a.B + b] = zz;
+                a.pt[split * a.B + b] = mine ? tl[n] : ot;
+                if (WITH_O) a.pd[split * a.B + b] = EVEN ? C : down_of(top[n], m[n]);
+            }
+            if constexpr (WITH_O) {
+                float *dst = a.po + (split * a.B + b) * DP;
+#pragma unroll
+                for (int q = 0; q < DB; ++q)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        *reinterpret_cast<float4 *>(dst + q * 32 + g * 8 + h * 4) =
+                            make_float4(o[q][n][4 * g], o[q][n][4 * g + 1], o[q][n][4 * g + 2], o[q][n][4 * g + 3]);
+            }
+        }
     };
-    copy_to_lds<TILE>(a.w.blocks + k0 * BLK, lds0, t);
-    copies_done();
-    __syncthreads();
-    for (int64_t k = k0; k < k1; k += 2) {
-        step(k, lds0, lds1);
-        if (k + 1 < k1) step(k + 1, lds1, lds0);
-    }
-    if (WITH_O && bt == 0 && t == 0) a.pc[split] = C;
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int64_t b = ((bt * 4 + wave) * NB + n) * kRB + col;
-        // the two halves of a row: same maximum, sums of different items, one target logit
-        const float zz = z[n] + __shfl_xor(z[n], 32, 64);
-        const float ot = __shfl_xor(tl[n], 32, 64);
-        const bool mine = (tgt[n] >> 2 & 1) == h;  // items 8q + 4h + 0..3 are this half's
-        if (!live[n] || b >= a.B) continue;
-        if (h == 0) {
-            a.pm[split * a.B + b] = m[n];
-            a.pz[split * a.B + b] = zz;
-            a.pt[split * a.B + b] = mine ? tl[n] : ot;
-        }
-        if constexpr (WITH_O) {
-            float *dst = a.po + (split * a.B + b) * DP;
-#pragma unroll
-            for (int q = 0; q < DB; ++q)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<float4 *>(dst + q * 32 + g * 8 + h * 4) =
-                        make_float4(o[q][n][4 * g], o[q][n][4 * g + 1], o[q][n][4 * g + 2], o[q][n][4 * g + 3]);
-        }
-    }
+    if (even) body(std::true_type());
+    if constexpr (P::kScaled)
+        if (!even) body(std::false_type());
 }
 
 struct JoinArgs {
     int64_t B, V, splits, per;
-    int32_t d, ooff;  // ooff: po carries 2^(ooff - C)
+    int32_t d, ooff;  // ooff: po carries 2^(ooff - pd)
     const float *pm, *pz, *pt, *po;
-    const int32_t *pc;
+    const int32_t *pd;
     const int64_t *target;
     int64_t ignore;
     float *loss, *lse2, *rest, *o;  // rest: r; o: [B, DP] or NULL
@@ -445,7 +540,7 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
     for (int c = 0; c < NC; ++c) acc[c] = 0.f;
 #pragma unroll 4
     for (int64_t s = q0; s < q1; ++s) {
-        const float f = __builtin_amdgcn_exp2f(a.pm[s * a.B + b] - m) * ldexpf(1.f, a.pc[s] - a.ooff);
+        const float f = ldexpf(__builtin_amdgcn_exp2f(a.pm[s * a.B + b] - m), a.pd[s * a.B + b] - a.ooff);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
             if (c * 64 + lane < DP) acc[c] = fmaf(a.po[(s * a.B + b) * DP + c * 64 + lane], f, acc[c]);
@@ -547,14 +642,14 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     if (a.per_row) {
         for (int64_t b = t; b < a.B; b += kThreads) {
             const float c = fabsf(row_coef(a, b, a.target[b]));
-            if (c > 0.f) c_all = max(c_all, block_exponent(c) + (SCALED ? a.x.exps[b / kRB] : 0));
+            if (c > 0.f) c_all = max(c_all, block_exponent(c) + (SCALED ? a.x.row_exps[b] : 0));
         }
     } else {  // one coefficient; blocks of nothing but ignored rows are packed as zeros and do not count
         const float c = a.grad[0] * a.scale / (a.mean ? fmaxf(*a.count, 1.f) : 1.f);
         const int e = block_exponent(fabsf(c));
         if (!SCALED) c_all = e;
         else
-            for (int64_t k = t; k < blocks_of(a.B); k += kThreads) c_all = max(c_all, e + a.x.exps[k]);
+            for (int64_t k = t; k < blocks_of(a.B); k += kThreads) c_all = max(c_all, e + largest_exp(a.x.exps[k]));
     }
     atomicMax(&cm, c_all);  // in LDS; a maximum does not depend on the order
     __syncthreads();
@@ -567,7 +662,7 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     if (b < a.B) {
         const int64_t tg = a.target[b];
         const float c = row_coef(a, b, tg);
-        const int e = SCALED ? a.x.exps[b / kRB] : 0;
+        const int e = SCALED ? a.x.row_exps[b] : 0;
         if (c != 0.f) {
             off = a.lse2[b] - log2f(fabsf(c)) - (float)(14 + e - C);
             hot = ldexpf(c * a.rest[b], 14 + e - C);
@@ -634,7 +729,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
         v0[n] = (int)(vs * kRB);
 #pragma unroll
         for (int k = 0; k < KS; ++k) load_frags<P>(a.w.blocks + vs * BLK, k, lane, wf[n][k]);
-        c_w[n] = a.scale2 * (P::kScaled ? pow2f(a.w.exps[vs] - P::kOff) : 1.f);
+        c_w[n] = a.scale2 * (P::kScaled ? pow2f(a.w.row_exps[vs * kRB + col] - P::kOff) : 1.f);
 #pragma unroll
         for (int q = 0; q < DB; ++q)
 #pragma unroll
@@ -652,7 +747,9 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
     int e_next = P::kScaled ? a.x.exps[k0] : 0, neg_next = a.info.neg[k0];
     auto step = [&](int64_t k, const u32x4_t *__restrict__ x, u32x4_t *__restrict__ next, const float (*info)[kRB],
                     float (*info_next)[kRB]) {
-        const float c_x = P::kScaled ? pow2f(__builtin_amdgcn_readfirstlane(e_next) - P::kOff) : 1.f;
+        const int e_k = P::kScaled ? __builtin_amdgcn_readfirstlane(e_next) : 0;
+        const int e_x = largest_exp(e_k);
+        const float c_x = P::kScaled ? pow2f(e_x - P::kOff) : 1.f;
         const bool neg = __builtin_amdgcn_readfirstlane(neg_next) != 0;
         float si = 0.f;
         if (k + 1 < k1) {
@@ -668,6 +765,11 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
             for (int i = 0; i < 16; ++i) acc[n][i] = 0.f;
         logits<P, KS, NB>(x, lane, [&](int n, int s) -> const Frags<P> & { return wf[n][s]; }, acc);
         // lane: item v0 + col; register i: batch row 8 (i/4) + 4 h + i%4 of the block
+        if (P::kScaled && is_wide(e_k))
+            each_exp(a.x.row_exps, k, h, [&](int i, int e) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) acc[n][i] = ldexpf(acc[n][i], e - e_x);
+            });
         const int tcol = __builtin_bit_cast(int, info[2][col]);
         Frags<P> pf[NB][2];
         Frags<P> rest[NB][P::NS == 1 ? 2 : 1];
@@ -821,7 +923,7 @@ FwdArgs fwd_args(Carve &c, int64_t b, int64_t v, int dp, bool with_o) {
     a.pm = c.take<float>(p.splits * b);
     a.pz = c.take<float>(p.splits * b);
     a.pt = c.take<float>(p.splits * b);
-    a.pc = c.take<int32_t>(p.splits);
+    a.pd = with_o ? c.take<int32_t>(p.splits * b) : nullptr;
     a.po = with_o ? c.take<float>(p.splits * b * dp) : nullptr;
     return a;
 }
@@ -847,7 +949,7 @@ using namespace igr;
 
 extern "C" int64_t igr_softmax_loss_pack_size(int64_t rows, int32_t d, int32_t dtype) {
     if (rows <= 0 || d <= 0 || d > 256 || dtype < kF32 || dtype > kF16) return 0;
-    return align256(blocks_of(rows) * (block_bytes(dtype, pad_width(d)) + (int64_t)sizeof(int32_t)));
+    return align256(blocks_of(rows) * (block_bytes(dtype, pad_width(d)) + (int64_t)sizeof(int32_t) + kRB));
 }
 
 extern "C" int64_t igr_softmax_loss_workspace_size(int64_t b, int64_t v, int32_t d, int32_t backward, int32_t with_o) {
@@ -883,9 +985,10 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
             const int64_t nx = blocks_of(b), nw = blocks_of(v), eb = dtype_bytes(dtype);
             const bool vec = d * eb % 16 == 0 && ldx * eb % 16 == 0 && ld_items * eb % 16 == 0 && aligned16(x) &&
                              aligned16(items);
-            PackArgs px{b, ldx, x, const_cast<u32x4_t *>(a.x.blocks), const_cast<int32_t *>(a.x.exps), target,
-                        ignore_index};
-            PackArgs pw{v, ld_items, items, const_cast<u32x4_t *>(a.w.blocks), const_cast<int32_t *>(a.w.exps), nullptr, 0};
+            PackArgs px{b, ldx, x, const_cast<u32x4_t *>(a.x.blocks), const_cast<int32_t *>(a.x.exps),
+                        const_cast<int8_t *>(a.x.row_exps), target, ignore_index};
+            PackArgs pw{v, ld_items, items, const_cast<u32x4_t *>(a.w.blocks), const_cast<int32_t *>(a.w.exps),
+                        const_cast<int8_t *>(a.w.row_exps), nullptr, 0};
             const FwdPlan plan = fwd_plan(b, v, dp);
             const int64_t grid = (a.splits + 7) / 8 * 8 * a.nbt;
             if (grid > INT32_MAX || nx + nw > INT32_MAX) return arg_error(fn, "too many workgroups");
@@ -905,7 +1008,7 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
                     if (o) hipLaunchKernelGGL((softmax_fwd<P, DP, 1, true>), g, dim3(kThreads), 0, st, a);
                     else hipLaunchKernelGGL((softmax_fwd<P, DP, 1, false>), g, dim3(kThreads), 0, st, a);
                 }
-                JoinArgs j{b, v, a.splits, a.per, d, 14 + P::kOff, a.pm, a.pz, a.pt, a.po, a.pc, target, ignore_index,
+                JoinArgs j{b, v, a.splits, a.per, d, 14 + P::kOff, a.pm, a.pz, a.pt, a.po, a.pd, target, ignore_index,
                            loss, lse2, lse2 + b, o};
                 hipLaunchKernelGGL((softmax_join<DP>), dim3((unsigned)b), dim3(kThreads), 0, st, j);
                 return IGR_OK;

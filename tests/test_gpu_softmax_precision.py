@@ -48,3 +48,149 @@ def test_half_type_gradients_are_rounded_once(B, V, d, dtype):
     tiny = 2.0 ** -25 if dtype == torch.float16 else 1e-37
     assert ((dx.double() - rx).abs() <= e[:, None] * mx + half * rx.abs() + floor + tiny).all()
     assert ((dw.double() - rw).abs() <= e.max() * mw + half * rw.abs() + floor + tiny).all()
+
+
+def pairwise(x, w, t, scale=1.0):
+    """As `reference` for fp32 tables, with the errors of each logit by its own terms: (loss, its bound, dx, its bound,
+    dw, its bound).  A logit is off by at most d_bv = (3 d + 16) 2^-24 sum_k |x_bk w_vk| (three products a term,
+    their rows held to 2^-23 whatever their neighbours are), a weight relative by d_bv, the row's mean of
+    these (its log-sum), 2^-20 and n 2^-24.  Below that there is a floor for each term of a gradient: a weight
+    times the power of two of its row is held to 2^-37 of the largest of these (of the row's in dx, where a
+    block's rows may share an exponent 2^8 above theirs; of the batch's in dw)."""
+    X, W = x.detach().double(), w.detach().double()
+    s = scale * X.matmul(W.t())
+    lse = torch.logsumexp(s, 1, keepdim=True)
+    p = (s - lse).exp()
+    at = torch.arange(len(t), device=x.device)
+    hot = torch.zeros_like(p)
+    hot[at, t] = 1.0
+    err = (3 * x.shape[1] + 16) * 2.0 ** -24 * scale * X.abs().matmul(W.abs().t())
+    mean = torch.where(p > 0, p * err, torch.zeros_like(p)).sum(1, keepdim=True)
+    n = 65 + max(x.shape[0], w.shape[0]) // 32
+    rel = err + mean + 2.0 ** -20 + n * 2.0 ** -24
+    loss = lse[:, 0] - s[at, t]
+    el = mean[:, 0] + err[at, t] + n * 2.0 ** -24 + 2.0 ** -22 * (loss.abs() + lse[:, 0].abs() + s[at, t].abs())
+    we = torch.where(p > 0, p * rel, torch.zeros_like(p)) + hot * (mean + 2.0 ** -20 + n * 2.0 ** -24)
+    top = (p * W.abs().amax(1)).amax(1, keepdim=True)
+    dx, dw = scale * (p - hot).matmul(W), scale * (p - hot).t().contiguous().matmul(X)
+    ex = scale * (we.matmul(W.abs()) + 2.0 ** -29 * w.shape[0] * top) + 2.0 ** -23 * dx.abs()
+    ew = scale * (we.t().contiguous().matmul(X.abs()) + 2.0 ** -37 * len(t) * X.abs().max()) + 2.0 ** -23 * dw.abs()
+    return loss, el, dx, ex, dw, ew
+
+
+def check_rows(x, w, t, scale=1.0, dx_columns=slice(None)):
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.softmax_loss(x, w, t, scale=scale, reduction='none')
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    rl, el, rx, ex, rw, ew = pairwise(x, w, t, scale)
+    assert ((loss.double() - rl).abs() <= el).all()
+    assert ((dx.double() - rx).abs() <= ex + 1e-37)[:, dx_columns].all()
+    assert ((dw.double() - rw).abs() <= ew + 1e-37).all()
+    with torch.no_grad():
+        assert torch.equal(loss, ops.softmax_loss(x, w, t, scale=scale, reduction='none'))
+
+
+def normal_tables(B, V, d, seed):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    std = (2.0 / d ** 0.5) ** 0.5
+    r = lambda n: std * torch.randn(n, d, generator=gen, device=DEV)  # noqa: E731
+    return r(B), r(V), torch.randint(0, V, (B,), generator=gen, device=DEV)
+
+
+@pytest.mark.parametrize('B,V,d', [(70, 300, 33), (200, 1000, 64), (40, 500, 100), (300, 260, 250)])
+@pytest.mark.parametrize('low', [-1e4, -1e9, torch.finfo(torch.float32).min])
+def test_items_masked_by_a_bias_column_leave_the_others_their_digits(B, V, d, low):
+    """A table with a bias column whose masked items hold a very low value, down to the type's lowest: they weigh
+    nothing, and the items that lie next to them are scored as if they were not there."""
+    x, w, t = normal_tables(B, V, d, B + d)
+    x[:, -1] = 1.0
+    w[:, -1] = 0.1
+    masked = torch.arange(0, V, 7, device=DEV)
+    w[masked, -1] = low
+    t = torch.where(t % 7 == 0, t + 1, t).clamp_(max=V - 1)
+    t[t % 7 == 0] = 1
+    check_rows(x, w, t)
+
+
+@pytest.mark.parametrize('B,V,d', [(70, 300, 33), (200, 1000, 64), (40, 500, 100)])
+@pytest.mark.parametrize('up', [9, 15, 25, 40, 100])
+def test_large_items_that_weigh_nothing_leave_the_others_their_digits(B, V, d, up):
+    """Items 2^up times the others' size in a direction that every batch row points away from: their weight
+    is nothing, and the weighted sums of the others hold their digits."""
+    x, w, t = normal_tables(B, V, d, B + up)
+    x[:, 0] = 1.5
+    w[:, 0] = 0.0
+    w[5::40] = 0.0
+    w[5::40, 0] = -2.0 ** up
+    w[6::80, 1] = 2.0 ** (up - 20)     # and some of another size
+    w[6::80, 0] = -2.0 ** up
+    t[(t % 40 == 5) | (t % 80 == 6)] = 0
+    check_rows(x, w, t)
+
+
+@pytest.mark.parametrize('up', [9, 15, 25])
+def test_large_batch_rows_leave_the_others_their_digits(up):
+    """Batch rows 2^up times the size of those beside them (at a scale that keeps their logits in range)."""
+    x, w, t = normal_tables(150, 400, 48, up)
+    x[::13] *= 2.0 ** up
+    check_rows(x, w, t, scale=2.0 ** (3 - up) if up > 12 else 1.0)
+    x, w, t = normal_tables(150, 400, 48, up + 1)
+    x[::13] *= 2.0 ** -up
+    w[::11] *= 2.0 ** -up
+    check_rows(x, w, t)
+
+
+def test_items_of_sizes_from_2_to_the_minus_60_to_2_to_the_60():
+    """Each row a size of its own, the large ones out of the batch rows' way."""
+    x, w, t = normal_tables(90, 640, 40, 3)
+    x[:, 0], w[:, 0] = 1.0, 0.0
+    e = (torch.arange(640, device=DEV) * 37 % 121 - 60).float()
+    w *= torch.exp2(e.clamp(max=0.0))[:, None]
+    w[:, 0] = -torch.exp2(e) * (e > 3)
+    t = torch.where(e[t] > 3, torch.zeros_like(t), t)
+    w[0] = 0.25
+    check_rows(x, w, t)
+
+
+def test_rows_of_their_own_size_in_a_long_table():
+    """Enough items for two blocks of them a wave in the backward, both tables with rows far from their neighbours."""
+    x, w, t = normal_tables(40, 140_000, 8, 5)
+    x[:, -1], w[:, -1] = 1.0, 0.0
+    x[::9] *= 2.0 ** -12
+    w[17::1000, -1] = -1e9
+    t = torch.where(t % 1000 == 17, t + 1, t)
+    check_rows(x, w, t)
+
+
+def test_ignored_rows_and_outside_targets_beside_masked_items():
+    x, w, t = normal_tables(100, 200, 24, 6)
+    x[:, -1], w[:, -1] = 1.0, 0.0
+    w[::5, -1] = -1e9
+    t = torch.where(t % 5 == 0, t + 1, t)
+    x.requires_grad_()
+    w.requires_grad_()
+    keep = torch.arange(100, device=DEV) % 3 != 0
+    ignored = torch.where(keep, t, torch.full_like(t, -100))
+    loss = ops.softmax_loss(x, w, ignored, reduction='none')
+    dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+    xs, ts = x.detach()[keep], t[keep]
+    rl, el, rx, ex, rw, ew = pairwise(xs, w, ts)
+    assert ((loss[keep].double() - rl).abs() <= el).all() and not loss[~keep].any()
+    assert ((dx[keep].double() - rx).abs() <= ex).all() and not dx[~keep].any()
+    assert ((dw.double() - rw).abs() <= ew).all()
+    out = t.clone()
+    out[7], out[50] = 200, -3
+    rows = ops.softmax_loss(x, w, out, reduction='none')
+    assert torch.isnan(rows[[7, 50]]).all() and int(torch.isnan(rows).sum()) == 2
+
+
+def test_blocks_of_zeros_are_even_with_any():
+    """Items of zeros (a padding row, a fresh table) have no size that others could differ from."""
+    x, w, t = normal_tables(150, 400, 40, 8)
+    w[32:96] = 0.0
+    w[100] = 0.0
+    x[64:96] = 0.0
+    check_rows(x, w, t)
+    check_rows(torch.zeros_like(x), w.detach().clone(), t)
+    check_rows(x.detach().clone(), torch.zeros_like(w), t)
