@@ -595,7 +595,10 @@ struct RowInfo {
     int32_t *tgt;
     int32_t *neg;   // per block: some c_b < 0
     int32_t *cmax;  // C: the largest e + floor(log2 |c_b|)
+    int32_t *part;  // kScanGroups partial maxima
 };
+constexpr int kScanGroups = 256;         // one partial maximum a thread of softmax_coef
+constexpr int64_t kScanInline = 8192;   // terms that every workgroup of softmax_coef goes through itself
 
 struct CoefArgs {
     int64_t B, V;
@@ -607,6 +610,7 @@ struct CoefArgs {
     Packed x;
     RowInfo info;
     int64_t n_info;    // workgroups that fill the row info (0: dw is not wanted)
+    int32_t scanned;   // info.part is filled
     const void *items; // for dx
     int64_t ld_items;
     void *dx;
@@ -617,6 +621,40 @@ __device__ __forceinline__ float row_coef(const CoefArgs &a, int64_t b, int64_t 
     if (tg < 0 || tg >= a.V) return NAN;
     const float g = (a.per_row ? a.grad[b] : a.grad[0]) * a.scale;
     return a.mean ? g / fmaxf(*a.count, 1.f) : g;
+}
+
+// A thread's share of C, terms first, first + stride, ...
+template <bool SCALED>
+__device__ __forceinline__ int scan_exponents(const CoefArgs &a, int64_t first, int64_t stride) {
+    int most = -250;
+    if (a.per_row) {
+        for (int64_t b = first; b < a.B; b += stride) {
+            const float c = fabsf(row_coef(a, b, a.target[b]));
+            if (c > 0.f) most = max(most, block_exponent(c) + (SCALED ? a.x.row_exps[b] : 0));
+        }
+    } else {  // one coefficient; blocks of nothing but ignored rows are packed as zeros and do not count
+        const float c = a.grad[0] * a.scale / (a.mean ? fmaxf(*a.count, 1.f) : 1.f);
+        const int e = block_exponent(fabsf(c));
+        if (!SCALED) return e;
+        for (int64_t k = first; k < blocks_of(a.B); k += stride) most = max(most, e + largest_exp(a.x.exps[k]));
+    }
+    return most;
+}
+inline int64_t scan_terms(int64_t b, bool per_row, bool scaled) { return per_row ? b : scaled ? blocks_of(b) : 1; }
+
+// C's partial maxima, for batches whose terms are too many for every workgroup of softmax_coef to go through: that
+// grows with the square of the batch.  A backward with a gradient for each row (V = 1024, d = 64, fp32) takes
+// 62 us at 8192 rows without this launch; at 16,384 rows 89 us without and 64 with it, at 65,536 237 and 111.
+template <bool SCALED>
+__global__ __launch_bounds__(kThreads) void softmax_scan(CoefArgs a) {
+    __shared__ int32_t wm[kThreads / 64];
+    const int t = threadIdx.x;
+    int most = scan_exponents<SCALED>(a, (int64_t)blockIdx.x * kThreads + t, (int64_t)kScanGroups * kThreads);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) most = max(most, __shfl_xor(most, o, 64));
+    if ((t & 63) == 0) wm[t >> 6] = most;
+    __syncthreads();
+    if (t == 0) a.info.part[blockIdx.x] = max(max(wm[0], wm[1]), max(wm[2], wm[3]));
 }
 
 // Workgroups below n_info: the row info of 256 rows.  The others: dx of four rows, one a wave.
@@ -638,19 +676,8 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     __shared__ int32_t cm;
     if (t == 0) cm = -250;
     __syncthreads();
-    int c_all = -250;
-    if (a.per_row) {
-        for (int64_t b = t; b < a.B; b += kThreads) {
-            const float c = fabsf(row_coef(a, b, a.target[b]));
-            if (c > 0.f) c_all = max(c_all, block_exponent(c) + (SCALED ? a.x.row_exps[b] : 0));
-        }
-    } else {  // one coefficient; blocks of nothing but ignored rows are packed as zeros and do not count
-        const float c = a.grad[0] * a.scale / (a.mean ? fmaxf(*a.count, 1.f) : 1.f);
-        const int e = block_exponent(fabsf(c));
-        if (!SCALED) c_all = e;
-        else
-            for (int64_t k = t; k < blocks_of(a.B); k += kThreads) c_all = max(c_all, e + largest_exp(a.x.exps[k]));
-    }
+    static_assert(kScanGroups == kThreads, "one partial maximum a thread");
+    const int c_all = a.scanned ? a.info.part[t] : scan_exponents<SCALED>(a, t, kThreads);
     atomicMax(&cm, c_all);  // in LDS; a maximum does not depend on the order
     __syncthreads();
     const int C = cm;
@@ -938,6 +965,7 @@ BwdArgs bwd_args(Carve &c, int64_t b, int64_t v, int dp) {
     a.info.tgt = c.take<int32_t>(rows);
     a.info.neg = c.take<int32_t>(rows / kRB);
     a.info.cmax = c.take<int32_t>(1);
+    a.info.part = c.take<int32_t>(kScanGroups);
     a.part = p.splits > 1 ? c.take<float>(p.splits * v * dp) : nullptr;
     return a;
 }
@@ -1048,14 +1076,16 @@ extern "C" int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t
         a.scale2 = scale * kLog2e;
         a.dw = dw;
         const FwdPlan plan = bwd_plan(b, v, dp);
+        const bool scan = dw && scan_terms(b, per_row != 0, dtype == kF32) > kScanInline;
         CoefArgs ca{b, v, d, per_row, mean, grad, count, lse2, lse2 + b, o, target, ignore_index, scale, a.x, a.info,
-                    dw ? (blocks_of(b) * kRB + kThreads - 1) / kThreads : 0, items, ld_items, dx};
+                    dw ? (blocks_of(b) * kRB + kThreads - 1) / kThreads : 0, (int32_t)scan, items, ld_items, dx};
         const int64_t cg = ca.n_info + (dx ? (b + 3) / 4 : 0);
         if (plan.splits > 65535 || plan.nbt > INT32_MAX) return arg_error(fn, "too many workgroups");
         const int rc = by_type_width(dtype, dp, [&](auto pol, auto width) -> int {
             using P = decltype(pol);
             using T = typename P::elem;
             constexpr int DP = decltype(width)::value;
+            if (scan) hipLaunchKernelGGL((softmax_scan<P::kScaled>), dim3(kScanGroups), dim3(kThreads), 0, st, ca);
             hipLaunchKernelGGL((softmax_coef<T, DP, P::kScaled>), dim3((unsigned)cg), dim3(kThreads), 0, st, ca);
             if (!dw) return IGR_OK;
             const dim3 g((unsigned)plan.nbt, (unsigned)plan.splits);

@@ -194,3 +194,52 @@ def test_blocks_of_zeros_are_even_with_any():
     check_rows(x, w, t)
     check_rows(torch.zeros_like(x), w.detach().clone(), t)
     check_rows(x.detach().clone(), torch.zeros_like(w), t)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('B', [8192, 8193, 70_000])
+def test_gradients_of_long_batches_with_one_for_each_row(B, dtype):
+    """The largest coefficient of the batch, which all rows' weights are held against, at any place of a batch that is
+    long enough for a pass of its own over them."""
+    gen = torch.Generator(device=DEV).manual_seed(B)
+    x = (0.5 * torch.randn(B, 16, generator=gen, device=DEV)).to(dtype).requires_grad_()
+    w = (0.5 * torch.randn(40, 16, generator=gen, device=DEV)).to(dtype).requires_grad_()
+    t = torch.randint(0, 40, (B,), generator=gen, device=DEV)
+    X, W = x.detach().double(), w.detach().double()
+    p = X.matmul(W.t()).softmax(1)
+    p[torch.arange(B, device=DEV), t] -= 1.0
+    loss = ops.softmax_loss(x, w, t, reduction='none')
+    for at in (0, B // 2, B - 1):
+        g = torch.randn(B, generator=gen, device=DEV)
+        g[at] = -2.0 ** 20
+        dx, dw = torch.autograd.grad(loss, (x, w), g, retain_graph=True)
+        c = p * g.double()[:, None]
+        rx, rw = c.matmul(W), c.t().contiguous().matmul(X)
+        half = HALF[dtype]
+        # 2^-15 stands for the sums' and weights' errors as in `reference`, relative to the terms' magnitudes
+        assert ((dx.double() - rx).abs() <= 2.0 ** -15 * c.abs().matmul(W.abs()) + half * rx.abs()).all()
+        assert ((dw.double() - rw).abs() <= 2.0 ** -15 * c.abs().t().contiguous().matmul(X.abs()) + half * rw.abs()).all()
+
+
+def test_the_backward_of_a_long_batch_takes_time_in_proportion():
+    """A gradient for each of 2^19 rows: a few hundred microseconds of work on 64 items.  (With every workgroup going through
+    the whole batch it took over ten times the backward of one gradient for all.)"""
+    B = 1 << 19
+    x, w = (torch.randn(n, 16, device=DEV, requires_grad=True) for n in (B, 64))
+    t = torch.randint(0, 64, (B,), device=DEV)
+    took = {}
+    for reduction in ('sum', 'none'):
+        loss = ops.softmax_loss(x, w, t, reduction=reduction)
+        g = torch.ones_like(loss)
+        for _ in range(3):
+            torch.autograd.grad(loss, (x, w), g, retain_graph=True)
+        times = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            torch.autograd.grad(loss, (x, w), g, retain_graph=True)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        took[reduction] = sorted(times)[2]
+    assert took['none'] < 3 * took['sum'] + 0.2, took
