@@ -41,6 +41,13 @@ inline int launch_status(const char *fn) {
     return IGR_OK;
 }
 
+// A launch holds fewer than 2^32 threads along a dimension: grids of 256-thread workgroups that may need more
+// go into a second one (flat_group() is the workgroup's number; a kernel leaves at once where it is n or above).
+constexpr int64_t kMaxGroups = (1ll << 24) - 1;
+inline dim3 flat_grid(int64_t n) {
+    return n <= kMaxGroups ? dim3((unsigned)n) : dim3(1u << 16, (unsigned)((n + (1 << 16) - 1) >> 16));
+}
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int kWave = 64;  // CDNA wavefront
@@ -124,6 +131,9 @@ __device__ __forceinline__ T ld_stream(const T *p) {
     return *p;
 }
 #endif
+
+// The number of a workgroup of a flat_grid.
+__device__ __forceinline__ int64_t flat_group() { return blockIdx.x + (int64_t)blockIdx.y * gridDim.x; }
 
 // Counter-based random numbers: splitmix64 finaliser of (seed, offset, index).
 // A draw is a pure function of its counters, so a kernel needs no RNG state

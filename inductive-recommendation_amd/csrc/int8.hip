@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(int64_t n, int32_t k, 
                                                           int64_t ldx, int8_t *__restrict__ q, int64_t ldq,
                                                           float *__restrict__ scale) {
     const int lane = threadIdx.x & (g - 1);
-    const int64_t row = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / g;
+    const int64_t row = (flat_group() * kThreads + threadIdx.x) / g;
     if (row >= n) return;  // whole groups leave together
     const T *xr = x + row * ldx;
     struct alignas(sizeof(T) * VE) Vec {
@@ -95,7 +95,7 @@ int launch_quantize(int64_t n, int32_t k, const void *x, int64_t ldx, int8_t *q,
     const int64_t grid = (n * g + kThreads - 1) / kThreads;
     if (grid > INT32_MAX) return arg_error("igr_quantize_rows", "too many rows");
     const T *xt = static_cast<const T *>(x);
-    const dim3 gr((unsigned)grid), b(kThreads);
+    const dim3 gr = flat_grid(grid), b(kThreads);
     if (vec) {
         if (g * ve * 2 >= k) hipLaunchKernelGGL((quantize_rows<T, V, 2>), gr, b, 0, st, n, k, g, xt, ldx, q, ldq, scale);
         else hipLaunchKernelGGL((quantize_rows<T, V, 8>), gr, b, 0, st, n, k, g, xt, ldx, q, ldq, scale);
@@ -341,7 +341,7 @@ int launch_mul(const char *fn, MulArgs g, hipStream_t st) {
         g.tm = (g.M + bm - 1) / bm;
         g.tn = (g.N + bn - 1) / bn;
         const int64_t n = (g.tm * g.tn + 7) / 8 * 8;
-        if (n > INT32_MAX) return arg_error(fn, "too many result tiles");
+        if (n > kMaxGroups) return arg_error(fn, "too many result tiles");
         hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(kThreads), 0, st, g);
         return launch_status(fn);
     };

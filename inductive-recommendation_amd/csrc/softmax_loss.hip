@@ -100,8 +100,9 @@ template <class P, int DP>
 __global__ __launch_bounds__(kThreads) void pack_rows(PackArgs a0, PackArgs a1, int64_t n0, int32_t d, int32_t vec) {
     __shared__ float tile[kRB][DP + 1];
     __shared__ uint32_t rmax[kRB];  // bits of the rows' largest finite magnitudes
-    const int64_t blk = blockIdx.x < n0 ? blockIdx.x : blockIdx.x - n0;
-    const PackArgs a = blockIdx.x < n0 ? a0 : a1;
+    const int64_t id = flat_group(), blk = id < n0 ? id : id - n0;
+    const PackArgs a = id < n0 ? a0 : a1;
+    if (blk * kRB >= a.rows) return;
     const typename P::elem *src = static_cast<const typename P::elem *>(a.src);
     const int64_t r0 = blk * kRB;
     const int t = threadIdx.x;
@@ -489,7 +490,8 @@ template <int DP>
 __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
     __shared__ float part[4][DP];
     __shared__ float wm[4], wz[4];
-    const int64_t b = blockIdx.x;
+    const int64_t b = flat_group();
+    if (b >= a.B) return;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int64_t tg = a.target[b];
     if (tg == a.ignore) {
@@ -661,9 +663,10 @@ __global__ __launch_bounds__(kThreads) void softmax_scan(CoefArgs a) {
 template <class T, int DP, bool SCALED>
 __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    if ((int64_t)blockIdx.x >= a.n_info) {
-        const int64_t b = ((int64_t)blockIdx.x - a.n_info) * 4 + wave;
-        if (b >= a.B) return;
+    const int64_t id = flat_group();
+    if (id >= a.n_info) {
+        const int64_t b = (id - a.n_info) * 4 + wave;
+        if (b >= a.B || !a.dx) return;
         const int64_t tg = a.target[b];
         const float c = row_coef(a, b, tg);
         const bool ok = tg != a.ignore;
@@ -681,7 +684,7 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     atomicMax(&cm, c_all);  // in LDS; a maximum does not depend on the order
     __syncthreads();
     const int C = cm;
-    const int64_t b = (int64_t)blockIdx.x * kThreads + t;
+    const int64_t b = id * kThreads + t;
     if (b >= blocks_of(a.B) * kRB) return;
     float off = INFINITY, hot = 0.f;
     int tgt = -1;
@@ -1019,11 +1022,11 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
                         const_cast<int8_t *>(a.w.row_exps), nullptr, 0};
             const FwdPlan plan = fwd_plan(b, v, dp);
             const int64_t grid = (a.splits + 7) / 8 * 8 * a.nbt;
-            if (grid > INT32_MAX || nx + nw > INT32_MAX) return arg_error(fn, "too many workgroups");
+            if (grid > kMaxGroups) return arg_error(fn, "too many batch rows for one launch");
             const int rc = by_type_width(dtype, dp, [&](auto pol, auto width) -> int {
                 using P = decltype(pol);
                 constexpr int DP = decltype(width)::value;
-                hipLaunchKernelGGL((pack_rows<P, DP>), dim3((unsigned)(nx + nw)), dim3(kThreads), 0, st, px, pw, nx, d,
+                hipLaunchKernelGGL((pack_rows<P, DP>), flat_grid(nx + nw), dim3(kThreads), 0, st, px, pw, nx, d,
                                    (int32_t)vec);
                 const dim3 g((unsigned)grid);
                 if constexpr (DP <= 64) {
@@ -1038,7 +1041,7 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
                 }
                 JoinArgs j{b, v, a.splits, a.per, d, 14 + P::kOff, a.pm, a.pz, a.pt, a.po, a.pd, target, ignore_index,
                            loss, lse2, lse2 + b, o};
-                hipLaunchKernelGGL((softmax_join<DP>), dim3((unsigned)b), dim3(kThreads), 0, st, j);
+                hipLaunchKernelGGL((softmax_join<DP>), flat_grid(b), dim3(kThreads), 0, st, j);
                 return IGR_OK;
             });
             if (rc) return rc;
@@ -1080,13 +1083,13 @@ extern "C" int igr_softmax_loss_bwd(int32_t dtype, int64_t b, int64_t v, int32_t
         CoefArgs ca{b, v, d, per_row, mean, grad, count, lse2, lse2 + b, o, target, ignore_index, scale, a.x, a.info,
                     dw ? (blocks_of(b) * kRB + kThreads - 1) / kThreads : 0, (int32_t)scan, items, ld_items, dx};
         const int64_t cg = ca.n_info + (dx ? (b + 3) / 4 : 0);
-        if (plan.splits > 65535 || plan.nbt > INT32_MAX) return arg_error(fn, "too many workgroups");
+        if (plan.splits > 65535 || plan.nbt > kMaxGroups) return arg_error(fn, "too many workgroups");
         const int rc = by_type_width(dtype, dp, [&](auto pol, auto width) -> int {
             using P = decltype(pol);
             using T = typename P::elem;
             constexpr int DP = decltype(width)::value;
             if (scan) hipLaunchKernelGGL((softmax_scan<P::kScaled>), dim3(kScanGroups), dim3(kThreads), 0, st, ca);
-            hipLaunchKernelGGL((softmax_coef<T, DP, P::kScaled>), dim3((unsigned)cg), dim3(kThreads), 0, st, ca);
+            hipLaunchKernelGGL((softmax_coef<T, DP, P::kScaled>), flat_grid(cg), dim3(kThreads), 0, st, ca);
             if (!dw) return IGR_OK;
             const dim3 g((unsigned)plan.nbt, (unsigned)plan.splits);
             if constexpr (DP <= 64) {

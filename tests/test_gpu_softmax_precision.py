@@ -243,3 +243,27 @@ def test_the_backward_of_a_long_batch_takes_time_in_proportion():
             times.append(a.elapsed_time(b))
         took[reduction] = sorted(times)[2]
     assert took['none'] < 3 * took['sum'] + 0.2, took
+
+
+def test_more_batch_rows_than_a_dimension_of_a_launch_has_workgroups():
+    """2^24 rows and more (a workgroup of 256 threads a row would pass 2^32 of them): the last ones are there."""
+    B, V, d = (1 << 24) + 77, 5, 4
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(B, d, generator=gen, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    w = torch.randn(V, d, generator=gen, device=DEV, dtype=torch.bfloat16).requires_grad_()
+    t = torch.randint(0, V, (B,), generator=gen, device=DEV)
+    loss = ops.softmax_loss(x, w, t, reduction='none')
+    g = torch.zeros(B, device=DEV)
+    some = torch.cat([torch.arange(100, device=DEV), torch.arange(B - 200, B, device=DEV)])
+    g[some] = 1.0
+    dx, dw = torch.autograd.grad(loss, (x, w), g)
+    X, W, T = x.detach()[some].double(), w.detach().double(), t[some]
+    p = X.matmul(W.t()).log_softmax(1)
+    at = torch.arange(len(some), device=DEV)
+    assert (loss.detach()[some].double() + p[at, T]).abs().max() < 1e-5
+    p = p.exp()
+    p[at, T] -= 1.0
+    rx, rw = p.matmul(W), p.t().contiguous().matmul(X)
+    assert ((dx[some].double() - rx).abs() <= 2.0 ** -8 * rx.abs() + 1e-4 * W.abs().max()).all()
+    assert ((dw.double() - rw).abs() <= 2.0 ** -8 * rw.abs() + 1e-4 * p.abs().t().contiguous().matmul(X.abs())).all()
+    assert not dx[100:B - 200].any()
