@@ -39,6 +39,9 @@ __device__ __forceinline__ void load2(const u32x4_t *p, int64_t frag, int lane, 
     f.p[1] = __builtin_bit_cast(half8_t, p[(frag * 2 + 1) * 64 + lane]);
 }
 
+// 1 / (|G| + eps); a matrix of zeros stays one, also with an eps of 0 or too small for its inverse.
+__device__ __forceinline__ double inverse_norm(double ss, double eps) { return ss == 0. ? 0. : 1. / (sqrt(ss) + eps); }
+
 // Four values as (hi, lo) halves.
 struct Quad {
     uint2 hi, lo;
@@ -111,7 +114,7 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
     if (lane == 0) red[wave] = ss;
     __syncthreads();
-    const double inv = 1. / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
+    const double inv = inverse_norm((red[0] + red[1]) + (red[2] + red[3]), eps);
     constexpr float up = 1 << kScale, down = 1.f / (1 << kScale);
     // values in x are X 2^11, as the fragments hold them
 #pragma unroll
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const do
     if (lane == 0) red[wave] = ss;
     __syncthreads();
     ss = (red[0] + red[1]) + (red[2] + red[3]);
-    const double inv = 1. / (sqrt(ss) + eps);
+    const double inv = inverse_norm(ss, eps);
     const T *src = g + batch * in.sb;
     const int64_t blk = (int64_t)blockIdx.x * 4 + wave;
     const int64_t r0 = blk / nb * 32, c0 = blk % nb * 32;
