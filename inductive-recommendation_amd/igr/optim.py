@@ -111,23 +111,24 @@ class Muon(Adam):
         if params and not isinstance(params[0], dict):
             params = [{'params': [p for p in params if p.dim() == 2], 'orthogonal': True},
                       {'params': [p for p in params if p.dim() != 2], 'orthogonal': False}]
-        groups = []
-        for g in params:
-            g = dict(g, params=list(g['params']) if not isinstance(g['params'], torch.Tensor) else [g['params']])
-            g.setdefault('orthogonal', False)
-            if g['orthogonal']:
-                g.setdefault('lr', orthogonal_lr)
-                for p in g['params']:
-                    if p.dim() != 2 or p.dtype != torch.float32:
-                        raise ValueError(f'Muon orthogonalises 2-D float32 weights, got {tuple(p.shape)} {p.dtype}')
-            if g['params']:
-                groups.append(g)
-        super().__init__(groups, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
-        for g in self.param_groups:
-            if g['orthogonal']:
-                for k, v in (('momentum', momentum), ('nesterov', nesterov), ('ns_steps', ns_steps),
-                             ('ns_coeffs', tuple(ns_coeffs))):
-                    g.setdefault(k, v)
+        self._orthogonal = dict(lr=orthogonal_lr, momentum=momentum, nesterov=nesterov, ns_steps=ns_steps,
+                                ns_coeffs=tuple(ns_coeffs))
+        groups = [dict(g, params=[g['params']] if isinstance(g['params'], torch.Tensor) else list(g['params'])) for g in params]
+        super().__init__([g for g in groups if g['params']], lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+
+    def add_param_group(self, param_group):
+        """Also what the constructor adds each of its groups with: 'orthogonal' (False if not given) decides the rule, and
+        with it which of the optimizer's settings the group takes where it names none."""
+        g = dict(param_group)
+        g['params'] = [g['params']] if isinstance(g['params'], torch.Tensor) else list(g['params'])
+        g.setdefault('orthogonal', False)
+        if g['orthogonal']:
+            for p in g['params']:
+                if p.dim() != 2 or p.dtype != torch.float32:
+                    raise ValueError(f'Muon orthogonalises 2-D float32 weights, got {tuple(p.shape)} {p.dtype}')
+            for k, v in self._orthogonal.items():
+                g.setdefault(k, v)
+        super().add_param_group(g)
 
     @classmethod
     def for_model(cls, model, **kw):
