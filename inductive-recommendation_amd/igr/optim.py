@@ -130,6 +130,18 @@ class Muon(Adam):
                 g.setdefault(k, v)
         super().add_param_group(g)
 
+    def load_state_dict(self, state_dict):
+        """Groups have to follow the rule that they were saved under (an Adam's, which names none, is Adam's).  Settings
+        that the saved groups lack stay this optimizer's."""
+        saved = []
+        for mine, group in zip(self.param_groups, state_dict['param_groups']):
+            if bool(group.get('orthogonal', False)) != bool(mine['orthogonal']):
+                raise ValueError('loaded state dict has a group under another rule (orthogonal: '
+                                 f"{bool(group.get('orthogonal', False))}, here {bool(mine['orthogonal'])})")
+            saved.append({**{k: v for k, v in mine.items() if k != 'params'}, **group})
+        saved += state_dict['param_groups'][len(saved):]
+        super().load_state_dict({**state_dict, 'param_groups': saved})
+
     @classmethod
     def for_model(cls, model, **kw):
         """Muon over a model's parameters: the weights of its nn.Linear layers orthogonalised, the rest Adam's."""

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from igr.optim import Muon
+from igr.optim import Adam, Muon
 
 SETTINGS = ('lr', 'momentum', 'nesterov', 'ns_steps', 'ns_coeffs')
 
@@ -32,6 +32,29 @@ def test_a_group_added_later_is_checked():
         with pytest.raises(ValueError, match='2-D float32'):
             opt.add_param_group({'params': [bad], 'orthogonal': True})
     assert len(opt.param_groups) == 1
+
+
+def test_a_state_saved_under_another_rule_is_refused():
+    p, q = weight(4, 4), weight(4, 4)
+    with pytest.raises(ValueError, match='another rule'):
+        Muon([p]).load_state_dict(Adam([q]).state_dict())
+    with pytest.raises(ValueError, match='another rule'):
+        Muon([{'params': [p]}]).load_state_dict(Muon([q]).state_dict())
+    with pytest.raises(ValueError, match='number of parameter groups'):
+        Muon([p]).load_state_dict(Muon([{'params': [q], 'orthogonal': True}, {'params': [weight(2, 2)]}]).state_dict())
+
+
+def test_an_adam_state_and_older_settings_load():
+    opt = Muon([{'params': [weight(4, 4)]}], lr=0.5)
+    opt.load_state_dict(Adam([weight(4, 4)], lr=0.25).state_dict())
+    assert opt.param_groups[0]['orthogonal'] is False and opt.param_groups[0]['lr'] == 0.25
+    state = Muon([weight(4, 4)], momentum=0.7).state_dict()
+    del state['param_groups'][0]['ns_steps']
+    kept = {k: v for k, v in state['param_groups'][0].items()}
+    opt = Muon([weight(4, 4)], ns_steps=2)
+    opt.load_state_dict(state)
+    assert opt.param_groups[0]['ns_steps'] == 2 and opt.param_groups[0]['momentum'] == 0.7
+    assert state['param_groups'][0] == kept
 
 
 @pytest.mark.gpu
