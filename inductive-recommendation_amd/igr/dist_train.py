@@ -466,11 +466,15 @@ class _LocalPairs:
 
 
 class ShardedIGCNTrainer:
-    """IGCNTrainer.step (trainer.py:531-561) on every rank of a sharded model."""
+    """IGCNTrainer.step (trainer.py:531-561) on every rank of a sharded model, with the reference's loss and optimizer
+    ('loss': 'softmax', 'optimizer': 'Muon' and 'score_dtype': 'int8' are the unsharded trainers')."""
 
     def __init__(self, trainer_config, model):
         from .optim import Adam
         from .sampler import DeviceBPRSampler
+        for key, only in (('loss', 'bpr'), ('optimizer', 'Adam'), ('score_dtype', 'float32')):
+            if trainer_config.get(key, only) != only:
+                raise ValueError(f'{key} {trainer_config[key]!r}: the sharded trainer has {only!r} alone')
         self.model = model
         self.config = trainer_config
         self.batch_size = trainer_config['batch_size']
