@@ -218,6 +218,9 @@ class LightGCN(BasicModel):
         return users_r, pos_r, neg_r, l2_norm_sq
 
     def predict(self, users, rep=None):
+        """The users' scores of every item.  rep: get_rep()'s, or its ops.QuantizedTable to score from 8-bit rows."""
+        if isinstance(rep, ops.QuantizedTable):
+            return ops.gemm_int8(*rep.rows(users), *rep.rows(slice(self.n_users, None)))
         rep = self.get_rep() if rep is None else rep
         users_r = ops.gather(rep, users)
         return ops.gemm(users_r, rep[self.n_users:])

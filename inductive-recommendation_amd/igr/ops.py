@@ -12,6 +12,7 @@ DGL-compatible surface (the reference's operator API):
     gspmm(g, 'copy_rhs', 'sum'|'max', None, e) ~ dgl.ops.gspmm   model.py:4270, 4273
     gsddmm(g, 'dot', lhs, rhs)                 ~ AttIGCN.masked_mm model.py:4246-4255
 """
+import collections
 import contextlib
 import ctypes
 import functools
@@ -1371,6 +1372,14 @@ def quantize_rows(x):
         scale = torch.empty(n, dtype=torch.float32, device=xs.device)
         L.call('igr_quantize_rows', dt, n, k, _p(xs), ldx, _p(q), ldq, _p(scale), _stream_of(xs.device))
     return (q if ldq == k else q[:, :k]), scale
+
+
+class QuantizedTable(collections.namedtuple('QuantizedTable', 'q scale')):
+    """quantize_rows' result as one table: what a model's predict takes in the place of rep to score from 8-bit rows."""
+    __slots__ = ()
+
+    def rows(self, index):
+        return QuantizedTable(self.q[index], self.scale[index])
 
 
 def gemm_int8(a, a_scale, b, b_scale, out_dtype=torch.float32):

@@ -25,7 +25,7 @@ every step, trainer.py:556).
 item against the whole catalogue at 'temperature' (default 1; model.softmax_loss) in place of the
 sampled BPR term, with the same l2 and aux terms beside it.  'score_dtype': 'float32'
 (default) or 'int8', evals ranked from 8-bit user and item rows (ops.quantize_rows once per eval,
-ops.gemm_int8 per batch).  'optimizer': 'Adam', or 'Muon' with 'orthogonal_lr' (default 0.02) for the
+ops.gemm_int8 per batch in the model's predict, which gets the ops.QuantizedTable as its rep).  'optimizer': 'Adam', or 'Muon' with 'orthogonal_lr' (default 0.02) for the
 weights of dense layers.
 """
 import contextlib
@@ -344,7 +344,8 @@ class BasicTrainer:
                              self.dataset.train_data, self.dataset.val_data)
             excl = cache[ck]
         kmax = max(self.topks)
-        predict = self._int8_predict(rep) if self.score_dtype == 'int8' else self.model.predict
+        if self.score_dtype == 'int8':  # once; a model whose predict knows no such table fails there
+            rep = ops.QuantizedTable(*ops.quantize_rows(rep))
         rec = []
         # test_batch_size bounds the reference's score matrix; rows are ranked
         # independently, so a batch sized for HBM (~1 GB of scores) gives the same
@@ -354,7 +355,7 @@ class BasicTrainer:
         for s in range(0, n_users, batch):
             e = min(n_users, s + batch)
             users = torch.arange(s, e, dtype=torch.int64, device=self.device)
-            scores = predict(users, rep)
+            scores = self.model.predict(users, rep)
             if excl is not None:
                 ops.mask_scores(scores, excl[0][s:e + 1], excl[1])
             if banned_items is not None:
@@ -363,15 +364,6 @@ class BasicTrainer:
             rec.append(items)  # stays on the device: one copy (and sync) per eval, not per batch
         rec = torch.cat(rec)
         return rec.cpu().numpy() if to_host else rec
-
-    def _int8_predict(self, rep):
-        """model.predict from the 8-bit rows of rep, quantised here once."""
-        q, scale = ops.quantize_rows(rep)
-        items = self.model.n_users
-
-        def predict(users, _):
-            return ops.gemm_int8(q[users], scale[users], q[items:], scale[items:])
-        return predict
 
     def eval(self, val_or_test, banned_items=None):
         """trainer.py:146-210; returns the reference's triple (result string,
