@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from igr import ops
+from test_pair_products import iterate, momentum, near_enough, off_by
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -24,3 +25,18 @@ def test_zeros_stay_zeros_whatever_eps_is(r, c, eps):
     g[1, 2, 3] = 1e-45   # the smallest there is
     y = ops.newton_schulz(g, eps=eps)
     assert not y[0].any() and torch.isfinite(y[1]).all() and 0.6 < float(y[1, 2, 3]) < 1.3
+
+
+SHAPES = [(1, 1), (1, 9), (7, 3), (64, 64), (64, 33), (5, 128), (64, 129), (256, 64), (33, 256), (64, 257), (65, 64), (65, 65),
+          (200, 520), (520, 200), (16, 4000), (1000, 130), (1100, 1030), (700, 900), (1030, 3001), (1500, 1100), (2304, 2304),
+          (300, 700), (40981, 64), (33, 9000), (20000, 100), (300000, 8)]
+
+
+@pytest.mark.parametrize('r,c', SHAPES)
+def test_as_near_as_pairs_of_halves_come(r, c):
+    """Within the bound that tells them from less (test_pair_products)."""
+    g = momentum(r, c).to(DEV)
+    y = ops.newton_schulz(g)
+    plain, exact = iterate(g, torch.float32), iterate(g, torch.float64)
+    assert near_enough(y, plain, exact), (off_by(y, exact), off_by(plain, exact))
+    print('off by %.3g, plain %.3g' % (off_by(y, exact), off_by(plain, exact)))

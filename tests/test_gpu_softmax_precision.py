@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from igr import ops
+from test_pair_products import loss_and_gradients, near_enough, off_by, tables
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -267,3 +268,19 @@ def test_more_batch_rows_than_a_dimension_of_a_launch_has_workgroups():
     assert ((dx[some].double() - rx).abs() <= 2.0 ** -8 * rx.abs() + 1e-4 * W.abs().max()).all()
     assert ((dw.double() - rw).abs() <= 2.0 ** -8 * rw.abs() + 1e-4 * p.abs().t().contiguous().matmul(X.abs())).all()
     assert not dx[100:B - 200].any()
+
+
+@pytest.mark.parametrize('B,V,d', [(3, 5, 7), (32, 32, 32), (33, 31, 64), (31, 33, 65), (129, 1000, 100), (256, 1682, 64),
+                                   (100, 70001, 32), (700, 333, 200), (64, 4097, 256), (300, 20000, 256), (2050, 300, 33),
+                                   (1, 5000, 129), (5000, 2, 16), (300, 140000, 24)])
+def test_as_near_as_pairs_of_halves_come(B, V, d):
+    """Losses row by row and both gradients, within the bound that tells pairs from less (test_pair_products)."""
+    x, w, t = (v.to(DEV) for v in tables(B, V, d))
+    x.requires_grad_()
+    w.requires_grad_()
+    loss = ops.softmax_loss(x, w, t, reduction='none')
+    got = (loss.detach(),) + torch.autograd.grad(loss.sum(), (x, w))
+    plain, exact = loss_and_gradients(x, w, t, torch.float32), loss_and_gradients(x, w, t, torch.float64)
+    for y, p, e in zip(got, plain, exact):
+        print('off by %.3g, plain %.3g' % (off_by(y, e), off_by(p, e)))
+        assert near_enough(y, p, e), (off_by(y, e), off_by(p, e))
