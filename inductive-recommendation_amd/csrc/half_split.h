@@ -108,7 +108,7 @@ __device__ __forceinline__ void split8(const float (&v)[8], Frags<SplitF32> &f) 
         f.p[1][i + 1] = l[1];
     }
 }
-// Half types: one rounding to nearest, half a step (2^-9 of the value for bf16, 2^-12 for fp16).
+// Half types: one rounding to nearest, off by at most half a step (2^-8 of the value for bf16, 2^-11 for fp16).
 __device__ __forceinline__ void split8(const float (&v)[8], Frags<PlainBF16> &f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f.p[0][i] = (__bf16)v[i];

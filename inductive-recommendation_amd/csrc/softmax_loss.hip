@@ -26,10 +26,15 @@
 // in registers and batch blocks streamed; no atomics on memory, the same bits on every run.
 //
 // Bound by the matrix cores and, beside them, the softmax's own arithmetic (an exponential, a
-// subtraction and two conversions a weight).  B = 2048, d = 64, fp32: one million items take 1.55 ms
-// forward and 1.3 ms backward, 1.1 to 1.25 PFLOP/s of fp16 products.  On operands that are not constant
+// subtraction and two conversions a weight).  B = 2048, d = 64, fp32: one million items take 1.54 ms
+// forward and 1.39 ms backward, 1.0 and 1.1 PFLOP/s of fp16 products.  On operands that are not constant
 // MFMAs alone sustain 1.56 here (2.3 on constants: the clock falls with what they switch), a large
-// library product 1.55.  40,981 items take 80 and 87 us.
+// library product 1.55.  40,981 items take 81 and 90 us; at d = 256 (one wave a SIMD) 0.35 and 0.31 ms
+// with the small kernels.
+//
+// fp32 in fewer bits than fp32's: operands are pairs of halves (2^-23, the rows' own powers of two), and an
+// exponent's argument, which log-sum, coefficient and power of two go into together, is one
+// fp32 of up to 40, so that a row's weights in dw share an error of up to 2^-20.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -201,8 +206,8 @@ __device__ __forceinline__ void load_frags(const u32x4_t *base, int f, int lane,
 
 // acc[n] += a streamed block's rows times the NB blocks of rows held in registers, over the width.  Four
 // steps' fragments are read from LDS before the first of their MFMAs: read one by one right before its
-// use, as the compiler orders them, each waits for LDS (1500 x 50,021 x 200 bf16: forward
-// 183 us, like this 170; at d = 64 the other workgroup covers most of it).
+// use, as the compiler orders them, each waits for LDS (1500 x 50,021 x 200 bf16, the kernel with weights
+// rounded once: 156 us, like this 148; at d = 64 the other workgroup covers most of it).
 template <class P, int KS, int NB, class B>
 __device__ __forceinline__ void logits(const u32x4_t *lds, int lane, const B &held, f32x16_t (&acc)[NB]) {
     constexpr int G = KS < 4 ? KS : 4;
@@ -223,7 +228,7 @@ __device__ __forceinline__ void logits(const u32x4_t *lds, int lane, const B &he
 // is off by half a step (2^-8 of it for bf16), and a sum of few large weights by as much.  1500 x 50,021 x
 // 200 in bf16: rounded once, the items' gradient, whose target's term often is nearly all there is, is off by
 // 2.8e-3 of its norm, as pairs by 1.7e-3, the result's own rounding; x's gradient differs from one of 32-bit
-// weights by 2.6e-4 and 9e-5 of its norm.  The second product costs the forward 160 -> 195 us.
+// weights by 2.6e-4 and 9e-5 of its norm.  The second product takes the forward's kernel from 148 to 187 us.
 template <class P, int NR>
 __device__ __forceinline__ void split_weights(float (&p)[16], Frags<P> (&w)[2], Frags<P> (&rest)[NR]) {
     float (&pl)[8] = reinterpret_cast<float (&)[8]>(p[0]);
@@ -891,7 +896,9 @@ struct FwdPlan {
     int64_t nbt, splits, per;
 };
 // Two blocks of batch rows a wave where they fit the registers of two workgroups on a CU and there
-// are that many rows: a streamed block then serves twice the rows.
+// are that many rows: a streamed block then serves twice the rows.  (Workgroups are counted over the whole chip, but
+// the kernel deals whole splits to the XCDs: few splits of a large batch leave XCDs idle.  65,536 rows
+// against 40,981 items of d = 64 are two splits, 7.1 ms forward beside 2.3 backward.)
 inline FwdPlan fwd_plan(int64_t B, int64_t V, int dp) {
     FwdPlan p;
     p.nb = dp <= 64 && B > 4 * kRB ? 2 : 1;
