@@ -253,9 +253,9 @@ struct FwdArgs {
 };
 
 // WITH_O = false: the loss alone (no product with the T part, which is then not copied either).
-// Two workgroups a CU wherever the registers do: all but fp32 rows of 256.
+// Two workgroups a CU wherever the registers do: all but o of fp32 rows of 256.
 template <class P, int DP, int NB, bool WITH_O>
-__global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax_fwd(FwdArgs a) {
+__global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) void softmax_fwd(FwdArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32;
     constexpr int TILE = block_halves<P>(DP) / 8 / (WITH_O ? 1 : 2);  // u32x4_t of a streamed block
     constexpr int BLK = block_halves<P>(DP) / 8;
