@@ -243,6 +243,16 @@ __device__ __forceinline__ void split_weights(float (&p)[16], Frags<P> (&w)[2], 
     }
 }
 
+// Logits (log2) beyond kFar take a path of their own: exp2(acc c - m), one fused operation, is off by the rounding of m
+// to fp32, which there is no small one (for a split of items that are all masked by -1e15 it is 2^25, and the
+// power infinite).
+constexpr float kFar = 512.f;
+// a b rounded to fp32, not to be fused with a difference: less a maximum that was rounded likewise it is 0 at most.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 struct FwdArgs {
     int64_t B, V, nbt, splits, per;  // batch tiles, catalogue splits, item blocks per split
     Packed x, w;
@@ -304,10 +314,10 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
         else asm volatile("; one exponent a row");
         // this wave's batch blocks
         Frags<P> xf[NB][KS];
-        // top: the largest log2 of a weight times its row's power of two so far
+        // top: the largest log2 of a weight (relative to m) times its row's power of two so far; far: some |m| is
         float c_x[NB], m[NB], top[NB], z[NB], tl[NB];
         int tgt[NB];
-        bool live[NB];
+        bool live[NB], far[NB];
         f32x16_t o[WITH_O ? DB : 1][NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -319,6 +329,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
             if constexpr (!P::kScaled) c_x[n] = a.scale2;
             else c_x[n] = a.scale2 * pow2f((EVEN ? largest_exp(a.x.exps[xs]) : a.x.row_exps[xs * kRB + col]) - P::kOff);
             m[n] = top[n] = -INFINITY;
+            far[n] = false;
             z[n] = 0.f;
             tl[n] = 0.f;
             const int64_t b = xs * kRB + col;
@@ -334,7 +345,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
         // (Two arrays by name, and the loop in pairs: so the compiler sees that reading one need not wait for
         // the copy into the other.)
         // o is held times 2^(14 - C or down) and its rows' 2^14: the largest product's weight is 2^14 in the halves' range
-        auto down_of = [](float top, float m) { return m > -INFINITY ? (int)ceilf(top - m) : 0; };
+        auto down_of = [](float top) { return top > -INFINITY ? (int)ceilf(top) : 0; };
         int ew_next = P::kScaled ? a.w.exps[k0] : 0;  // loaded a block ahead, before that block's copy is begun
         auto step = [&](int64_t k, const u32x4_t *__restrict__ w, u32x4_t *__restrict__ next) __attribute__((always_inline)) {
             const int ew = P::kScaled ? largest_exp(__builtin_amdgcn_readfirstlane(ew_next)) : 0;
@@ -380,23 +391,26 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
 #pragma unroll
                 for (int i = 1; i < 16; ++i) mx = fmaxf(mx, acc[n][i]);
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-                float mt = -INFINITY;  // the largest log2 of the block's weights times their rows' powers of two
+                const float mn = fmaxf(m[n], mx), base = mn == -INFINITY ? 0.f : mn;  // (none yet but the target)
+                float mt = -INFINITY;  // of the block's weights times their rows' powers of two the largest log2
                 if constexpr (!EVEN) {
-                    each_exp(a.w.row_exps, k, h, [&](int i, int e) { mt = fmaxf(mt, fmaf(acc[n][i], c, (float)e)); });
+                    each_exp(a.w.row_exps, k, h, [&](int i, int e) {
+                        mt = fmaxf(mt, rounded_product(acc[n][i], c) - base + (float)e);
+                    });
                     mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
                 }
                 if (__any(mx > m[n] || (!EVEN && mt > top[n]))) {  // rare after the first blocks
-                    const float mn = fmaxf(m[n], mx);
                     const float less = m[n] == mn ? 0.f : m[n] - mn;  // (both may be -infinity)
                     const float f = __builtin_amdgcn_exp2f(less);
                     z[n] *= f;
                     float fo = f;
                     if constexpr (!EVEN) {
-                        const float tn = fmaxf(top[n], mt);
-                        fo = __builtin_amdgcn_exp2f(less + (float)(down_of(top[n], m[n]) - down_of(tn, mn)));
+                        const float tn = fmaxf(top[n] + less, mt);
+                        fo = __builtin_amdgcn_exp2f(less + (float)(down_of(top[n]) - down_of(tn)));
                         top[n] = tn;
                     }
                     m[n] = mn;
+                    far[n] = __any(fabsf(base) > kFar);
                     if constexpr (WITH_O) {
 #pragma unroll
                         for (int q = 0; q < DB; ++q)
@@ -409,11 +423,16 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
                 // below adds nothing to o either way.
                 // (without o the same powers, for the same sums bit for bit)
                 const int sh = EVEN ? 14 + (P::kScaled ? max(ew - C, -60) : 0) : 0;
-                // (no maximum yet: the target is the only item so far)
-                const float off = m[n] == -INFINITY ? 0.f : m[n] - (float)sh;
                 float p[16];
+                if (!EVEN || far[n]) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
+                    for (int i = 0; i < 16; ++i)
+                        p[i] = ldexpf(__builtin_amdgcn_exp2f(rounded_product(acc[n][i], c) - base), sh);
+                } else {
+                    const float off = base - (float)sh;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(acc[n][i], c, -off));
+                }
                 float s0 = 0.f, s1 = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
@@ -423,7 +442,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
                 z[n] = fmaf(s0 + s1, pow2f(-sh), z[n]);
                 if constexpr (WITH_O) {
                     if constexpr (!EVEN) {  // each weight by its own row's power, up to 2^14 again
-                        const int up = 14 - down_of(top[n], m[n]);
+                        const int up = 14 - down_of(top[n]);
                         each_exp(a.w.row_exps, k, h, [&](int i, int e) { p[i] = ldexpf(p[i], e + up); });
                     }
                     split_weights<P>(p, pf[n], rest[n]);
@@ -461,7 +480,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
                 a.pm[split * a.B + b] = m[n];
                 a.pz[split * a.B + b] = zz;
                 a.pt[split * a.B + b] = mine ? tl[n] : ot;
-                if (WITH_O) a.pd[split * a.B + b] = EVEN ? C : down_of(top[n], m[n]);
+                if (WITH_O) a.pd[split * a.B + b] = EVEN ? C : down_of(top[n]);
             }
             if constexpr (WITH_O) {
                 float *dst = a.po + (split * a.B + b) * DP;
@@ -550,7 +569,10 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
         const float f = ldexpf(__builtin_amdgcn_exp2f(a.pm[s * a.B + b] - m), a.pd[s * a.B + b] - a.ooff);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-            if (c * 64 + lane < DP) acc[c] = fmaf(a.po[(s * a.B + b) * DP + c * 64 + lane], f, acc[c]);
+            if (c * 64 + lane < DP) {
+                const float v = a.po[(s * a.B + b) * DP + c * 64 + lane];
+                acc[c] = f == 0.f ? acc[c] : fmaf(v, f, acc[c]);  // (of items that are all masked v may be infinite)
+            }
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)

@@ -284,3 +284,62 @@ def test_as_near_as_pairs_of_halves_come(B, V, d):
     for y, p, e in zip(got, plain, exact):
         print('off by %.3g, plain %.3g' % (off_by(y, e), off_by(p, e)))
         assert near_enough(y, p, e), (off_by(y, e), off_by(p, e))
+
+
+LOWS = {torch.float32: [-1e5, -1e9, -1e15, -3e38], torch.bfloat16: [-1e5, -1e9, -1e15, -3e38], torch.float16: [-6e4]}
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('B,V,d,lo,hi', [(2, 34, 2, 32, 34), (40, 5000, 24, 1000, 3300), (200, 3000, 64, 64, 2990),
+                                         (60, 900, 130, 5, 870)])
+def test_a_range_of_masked_items(B, V, d, lo, hi, dtype):
+    """Whole stretches of the catalogue masked by a bias column, all that some workgroups see: logits of
+    down to -3e38, whose fp32 steps are far above 1."""
+    for low in LOWS[dtype]:
+        for scale in (0.3, 1.0, 2.0):
+            x, w, t = normal_tables(B, V, d, B + V)
+            x[:, -1], w[:, -1] = 1.0, 0.0
+            w[lo:hi, -1] = low
+            t = torch.where((t >= lo) & (t < hi), t % lo, t)
+            if dtype == torch.float32:
+                check_rows(x, w, t, scale=scale)
+                continue
+            x, w = x.to(dtype).requires_grad_(), w.to(dtype).requires_grad_()
+            loss = ops.softmax_loss(x, w, t, scale=scale, reduction='none')
+            dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+            rl, el, rx, ex, rw, ew = pairwise(x.detach().float(), w.detach().float(), t, scale)
+            half, tiny = HALF[dtype], 2.0 ** -25 if dtype == torch.float16 else 1e-37
+            assert ((loss.double() - rl).abs() <= el).all()
+            weights = half * half   # as pairs: twice the type's digits, of the terms' magnitudes
+            p = (scale * x.detach().double().matmul(w.detach().double().t())).softmax(1)
+            p[torch.arange(B, device=DEV), t] += 1.0
+            mx, mw = scale * p.matmul(w.detach().double().abs()), scale * p.t().contiguous().matmul(x.detach().double().abs())
+            assert ((dx.double() - rx).abs() <= ex + weights * mx + half * rx.abs() + tiny).all()
+            assert ((dw.double() - rw).abs() <= ew + weights * mw + half * rw.abs() + tiny).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('size', [2.0 ** 12, 2.0 ** 20, 2.0 ** 40, 2.0 ** 80])
+def test_losses_of_large_logits(size, dtype):
+    """Logits that fp32 holds exactly, in steps of their own size: equal ones share the weight, others have none."""
+    B, V, d = 50, 300, 6
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    w = torch.zeros(V, d, device=DEV)
+    w[:, 0] = torch.randint(-3, 3, (V,), generator=gen, device=DEV).float()
+    w[:, 1] = torch.randn(V, generator=gen, device=DEV)
+    x = torch.zeros(B, d, device=DEV)
+    x[:, 0] = size
+    x[25:, 0] = -size
+    x, w = x.to(dtype).requires_grad_(), w.to(dtype).requires_grad_()
+    t = torch.randint(0, V, (B,), generator=gen, device=DEV)
+    loss = ops.softmax_loss(x, w, t, reduction='none')
+    dx, = torch.autograd.grad(loss.sum(), x, retain_graph=True)
+    X, W = x.detach().double(), w.detach().double()
+    s = X.matmul(W.t())
+    top = s.amax(1, keepdim=True)   # (a log-sum of 2^42 has steps of 2^-11 in 64 bits too)
+    ref = (s - top).exp().sum(1).log() + (top - s.gather(1, t[:, None]))[:, 0]
+    assert ((loss.double() - ref).abs() <= 2.0 ** -20 * ref.abs() + 2.0 ** -20 * 8).all()
+    p = s.softmax(1)
+    p[torch.arange(B, device=DEV), t] -= 1.0
+    rx = p.matmul(W)
+    assert ((dx.double() - rx).abs() <= HALF[dtype] * rx.abs() + 2.0 ** -16 * p.abs().matmul(W.abs()) + 1e-6).all()
