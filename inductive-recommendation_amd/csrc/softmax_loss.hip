@@ -58,7 +58,7 @@ __host__ __device__ constexpr int block_halves(int dp) { return 2 * P::NS * kRB 
 inline int64_t block_bytes(int32_t dtype, int dp) { return (dtype == kF32 ? 2 : 1) * 2ll * kRB * dp * 2; }
 inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
 
-// A packed table: its blocks, then fp32's exponents: a row's entries are held times 2^(14 - its own).  A block
+// A packed table: its blocks, then (of the batch) what fp32 leaves of the rows' log-sums, and fp32's exponents: a row's entries are held times 2^(14 - its own).  A block
 // whose rows are within 2^kNarrow of each other has one exponent for all of them (its largest row's), and
 // the kernels their short path; the digits of a row 2^8 below it still reach 2^-31 of its largest entry.  In
 // the others each row has its own, however large its neighbours are (an item masked by
@@ -67,12 +67,19 @@ struct Packed {
     const u32x4_t *blocks;
     const int32_t *exps;      // per block: its largest row's, plus kWide where rows have their own
     const int8_t *row_exps;   // per row, padded to whole blocks
+    const int16_t *lse_rest;  // per row, in units of rest_unit(lse2)
 };
 constexpr int kNarrow = 8, kWide = 1024, kZeros = -101;  // kZeros: a block of zeros
 inline Packed packed_view(const void *p, int64_t rows, int32_t dtype, int dp) {
     const char *c = static_cast<const char *>(p) + blocks_of(rows) * block_bytes(dtype, dp);
     return Packed{static_cast<const u32x4_t *>(p), reinterpret_cast<const int32_t *>(c),
-                  reinterpret_cast<const int8_t *>(c + blocks_of(rows) * sizeof(int32_t))};
+                  reinterpret_cast<const int8_t *>(c + blocks_of(rows) * sizeof(int32_t)),
+                  reinterpret_cast<const int16_t *>(c + blocks_of(rows) * (sizeof(int32_t) + kRB))};
+}
+// lse2 is off by half its fp32 step at most, and by no more than the log of a sum, below 32: 2^-15 of that.
+__device__ __forceinline__ float rest_unit(float lse2) {
+    const int step = (int)((__builtin_bit_cast(uint32_t, lse2) >> 23) & 255u) - 127 - 24;  // of half a step
+    return ldexpf(1.f, min(step, 5) - 15);
 }
 __host__ __device__ inline int largest_exp(int e) { return e >= kWide / 2 ? e - kWide : e; }
 __host__ __device__ inline bool is_wide(int e) { return e >= kWide / 2; }
@@ -506,6 +513,7 @@ struct JoinArgs {
     const int64_t *target;
     int64_t ignore;
     float *loss, *lse2, *rest, *o;  // rest: r; o: [B, DP] or NULL
+    int16_t *lse_rest;
 };
 
 // One batch row per workgroup: the splits' (max, sum, o) joined in split order, a quarter of them
@@ -522,6 +530,7 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
         if (t == 0) {
             a.loss[b] = 0.f;
             a.lse2[b] = 0.f;
+            a.lse_rest[b] = 0;
             a.rest[b] = 0.f;
         }
         if (a.o)
@@ -555,7 +564,9 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
     }
     if (t == 0) {
         a.loss[b] = loss;
-        a.lse2[b] = m + log2f(z);
+        const float l = log2f(z), lse = m + l;
+        a.lse2[b] = lse;
+        a.lse_rest[b] = (int16_t)fminf(fmaxf(rintf(((m - lse) + l) / rest_unit(lse)), -32767.f), 32767.f);
         a.rest[b] = others / z;
     }
     if (!a.o) return;
@@ -622,10 +633,12 @@ __global__ __launch_bounds__(kReduceThreads) void softmax_reduce(int64_t B, cons
 struct RowInfo {
     float *off, *hot;
     int32_t *tgt;
-    int32_t *neg;   // per block: some c_b < 0
+    int32_t *flags; // per block: kMinus, some c_b < 0; kFarRows, some |lse2| > kFar
+    float2 *apart;  // lse2 as it is, and what off has beside it
     int32_t *cmax;  // C: the largest e + floor(log2 |c_b|)
     int32_t *part;  // kScanGroups partial maxima
 };
+constexpr int kMinus = 1, kFarRows = 2;
 constexpr int kScanGroups = 256;         // one partial maximum a thread of softmax_coef
 constexpr int64_t kScanInline = 8192;   // terms that every workgroup of softmax_coef goes through itself
 
@@ -715,13 +728,17 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     if (b >= blocks_of(a.B) * kRB) return;
     float off = INFINITY, hot = 0.f;
     int tgt = -1;
-    bool minus = false;
+    bool minus = false, far = false;
+    float2 apart = make_float2(0.f, -INFINITY);
     if (b < a.B) {
         const int64_t tg = a.target[b];
         const float c = row_coef(a, b, tg);
         const int e = SCALED ? a.x.row_exps[b] : 0;
         if (c != 0.f) {
-            off = a.lse2[b] - log2f(fabsf(c)) - (float)(14 + e - C);
+            const float lse = a.lse2[b], rest = log2f(fabsf(c)) + (float)(14 + e - C);
+            off = lse - rest;
+            far = fabsf(lse) > kFar;
+            apart = make_float2(lse, rest - (float)a.x.lse_rest[b] * rest_unit(lse));
             hot = ldexpf(c * a.rest[b], 14 + e - C);
             minus = c < 0.f;
             tgt = tg >= 0 && tg < a.V ? (int)tg : -1;
@@ -730,8 +747,10 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     a.info.off[b] = off;
     a.info.hot[b] = hot;
     a.info.tgt[b] = tgt;
-    const uint64_t neg = __ballot(minus);
-    if ((lane & 31) == 0) a.info.neg[b / kRB] = (uint32_t)(neg >> lane) != 0;
+    a.info.apart[b] = apart;
+    const uint64_t neg = __ballot(minus), wide = __ballot(far);
+    if ((lane & 31) == 0)
+        a.info.flags[b / kRB] = ((uint32_t)(neg >> lane) ? kMinus : 0) | ((uint32_t)(wide >> lane) ? kFarRows : 0);
     if (b == 0) *a.info.cmax = C;
 }
 
@@ -801,17 +820,18 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
         else if (t < 3 * kRB) v = __builtin_bit_cast(float, a.info.tgt[k * kRB + t - 2 * kRB]);
         return v;
     };
-    int e_next = P::kScaled ? a.x.exps[k0] : 0, neg_next = a.info.neg[k0];
+    int e_next = P::kScaled ? a.x.exps[k0] : 0, flags_next = a.info.flags[k0];
     auto step = [&](int64_t k, const u32x4_t *__restrict__ x, u32x4_t *__restrict__ next, const float (*info)[kRB],
                     float (*info_next)[kRB]) {
         const int e_k = P::kScaled ? __builtin_amdgcn_readfirstlane(e_next) : 0;
         const int e_x = largest_exp(e_k);
         const float c_x = P::kScaled ? pow2f(e_x - P::kOff) : 1.f;
-        const bool neg = __builtin_amdgcn_readfirstlane(neg_next) != 0;
+        const int flags = __builtin_amdgcn_readfirstlane(flags_next);
+        const bool neg = flags & kMinus;
         float si = 0.f;
         if (k + 1 < k1) {
             if (P::kScaled) e_next = a.x.exps[k + 1];
-            neg_next = a.info.neg[k + 1];
+            flags_next = a.info.flags[k + 1];
             si = fetch_info(k + 1);
             copy_to_lds<BLK>(a.x.blocks + (k + 1) * BLK, next, t);
         }
@@ -834,6 +854,14 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
         for (int n = 0; n < NB; ++n) {
             const float c = c_w[n] * c_x;
             float p[16];
+            if (flags & kFarRows) {  // equal logits as in the forward: one less the other is 0
+                const volatile float2 *apart = a.info.apart + k * kRB + 4 * h;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float lse = apart[8 * (i >> 2) + (i & 3)].x, rest = apart[8 * (i >> 2) + (i & 3)].y;
+                    p[i] = __builtin_amdgcn_exp2f((rounded_product(acc[n][i], c) - lse) + rest);
+                }
+            } else
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float4 off = *reinterpret_cast<const float4 *>(&info[0][8 * g + 4 * h]);
@@ -995,7 +1023,8 @@ BwdArgs bwd_args(Carve &c, int64_t b, int64_t v, int dp) {
     a.info.off = c.take<float>(rows);
     a.info.hot = c.take<float>(rows);
     a.info.tgt = c.take<int32_t>(rows);
-    a.info.neg = c.take<int32_t>(rows / kRB);
+    a.info.flags = c.take<int32_t>(rows / kRB);
+    a.info.apart = c.take<float2>(rows);
     a.info.cmax = c.take<int32_t>(1);
     a.info.part = c.take<int32_t>(kScanGroups);
     a.part = p.splits > 1 ? c.take<float>(p.splits * v * dp) : nullptr;
@@ -1009,7 +1038,7 @@ using namespace igr;
 
 extern "C" int64_t igr_softmax_loss_pack_size(int64_t rows, int32_t d, int32_t dtype) {
     if (rows <= 0 || d <= 0 || d > 256 || dtype < kF32 || dtype > kF16) return 0;
-    return align256(blocks_of(rows) * (block_bytes(dtype, pad_width(d)) + (int64_t)sizeof(int32_t) + kRB));
+    return align256(blocks_of(rows) * (block_bytes(dtype, pad_width(d)) + (int64_t)sizeof(int32_t) + 3 * kRB));
 }
 
 extern "C" int64_t igr_softmax_loss_workspace_size(int64_t b, int64_t v, int32_t d, int32_t backward, int32_t with_o) {
@@ -1069,7 +1098,8 @@ extern "C" int igr_softmax_loss_fwd(int32_t dtype, int64_t b, int64_t v, int32_t
                     else hipLaunchKernelGGL((softmax_fwd<P, DP, 1, false>), g, dim3(kThreads), 0, st, a);
                 }
                 JoinArgs j{b, v, a.splits, a.per, d, 14 + P::kOff, a.pm, a.pz, a.pt, a.po, a.pd, target, ignore_index,
-                           loss, lse2, lse2 + b, o};
+                           loss, lse2, lse2 + b, o,
+                           const_cast<int16_t *>(a.x.lse_rest)};
                 hipLaunchKernelGGL((softmax_join<DP>), flat_grid(b), dim3(kThreads), 0, st, j);
                 return IGR_OK;
             });

@@ -343,3 +343,36 @@ def test_losses_of_large_logits(size, dtype):
     p[torch.arange(B, device=DEV), t] -= 1.0
     rx = p.matmul(W)
     assert ((dx.double() - rx).abs() <= HALF[dtype] * rx.abs() + 2.0 ** -16 * p.abs().matmul(W.abs()) + 1e-6).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('size', [2.0 ** 7, 2.0 ** 9, 2.0 ** 12, 2.0 ** 17, 2.0 ** 23, 2.0 ** 40, 2.0 ** 80])
+@pytest.mark.parametrize('reduction', ['sum', 'none'])
+def test_items_gradients_of_large_logits(size, dtype, reduction):
+    """As above, beside rows of small logits in the same blocks.  The log-sum of such a row is kept to 2^-16 of half its
+    fp32 step, or of 32 where that is less (steps from 2^6 on): a weight is off by 2^-11 at most for that, 2^-16 for
+    the rest."""
+    B, V, d = 90, 300, 6
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    w = torch.zeros(V, d, device=DEV)
+    w[:, 0] = torch.randint(-3, 3, (V,), generator=gen, device=DEV).float()
+    w[:, 1] = torch.randn(V, generator=gen, device=DEV)
+    x = torch.zeros(B, d, device=DEV)
+    x[:, 0] = size
+    x[30:, 0] = -size
+    x[::3, 0], x[::3, 1] = 0.0, 1.0
+    x, w = x.to(dtype).requires_grad_(), w.to(dtype).requires_grad_()
+    t = torch.randint(0, V, (B,), generator=gen, device=DEV)
+    loss = ops.softmax_loss(x, w, t, reduction=reduction)
+    g = torch.ones_like(loss) if reduction == 'sum' else torch.randn(B, generator=gen, device=DEV)
+    dw, = torch.autograd.grad(loss, w, g)
+    X, W = x.detach().double(), w.detach().double()
+    s = X.matmul(W.t())
+    p = (s - s.amax(1, keepdim=True)).softmax(1)
+    p[torch.arange(B, device=DEV), t] -= 1.0
+    p = p * (g.double()[:, None] if reduction == 'none' else 1.0)
+    rw = p.t().contiguous().matmul(X)
+    terms = p.abs().t().contiguous().matmul(X.abs())
+    floor = 2.0 ** -37 * B * float(X.abs().max()) * float(g.abs().max())
+    off = (2.0 ** -11 if size >= 2.0 ** 17 else 0.0) + 2.0 ** -16
+    assert ((dw.double() - rw).abs() <= off * terms + HALF[dtype] * rw.abs() + floor).all()
