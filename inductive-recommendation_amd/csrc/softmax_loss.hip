@@ -578,11 +578,14 @@ __global__ __launch_bounds__(kThreads) void softmax_join(JoinArgs a) {
 #pragma unroll 4
     for (int64_t s = q0; s < q1; ++s) {
         const float f = ldexpf(__builtin_amdgcn_exp2f(a.pm[s * a.B + b] - m), a.pd[s * a.B + b] - a.ooff);
+        // (of items that are all masked po may be infinite: 0 in its place, by its bits, for a load under a condition
+        // takes the kernel from 11 to 16 us)
+        const uint32_t bits = f == 0.f ? 0u : ~0u;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
             if (c * 64 + lane < DP) {
                 const float v = a.po[(s * a.B + b) * DP + c * 64 + lane];
-                acc[c] = f == 0.f ? acc[c] : fmaf(v, f, acc[c]);  // (of items that are all masked v may be infinite)
+                acc[c] = fmaf(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & bits), f, acc[c]);
             }
     }
 #pragma unroll
