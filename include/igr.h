@@ -598,8 +598,8 @@ int igr_gemm_int8(int64_t m, int64_t n, int32_t k, const int8_t *a, int64_t lda,
  * stride_g elements apart; unit inner stride) of `dtype` into out [batch, rows, cols]:
  *   X = G / (|G|_F + eps),   steps times:  A = X X^T,  X <- a X + (b A + c A A) X
  * (X^T X for rows > cols).  The iteration is carried in fp32 accuracy whatever the type, one
- * rounding at the end.  Coefficients that would take a singular value of [0, 1] above 4
- * on the way are refused.  A matrix of zeros gives zeros, one with an infinity or NaN NaN.
+ * rounding at the end, however small |G| is beside eps.  Coefficients that would take a singular value of
+ * [0, 1] above 4 on the way are refused.  A matrix of zeros gives zeros, one with an infinity or NaN NaN.
  * The workspace holds igr_newton_schulz_workspace_size bytes (0 for matrices within 64 x 256). */
 int64_t igr_newton_schulz_workspace_size(int64_t batch, int64_t rows, int64_t cols);
 int igr_newton_schulz(int32_t dtype, int64_t batch, int64_t rows, int64_t cols, const void *g, int64_t ldg,

@@ -6,6 +6,8 @@
 // is held as pairs of halves (half_split.h) and multiplied in three 16-bit products.  X's
 // singular values stay below about 1.2 and A's and b A + c A A's entries below 3, so one
 // fixed scale 2^11 serves all of them: entries up to 32, down to steps of 2^-35.
+// Where |G| is not above eps, X_0 is small: X is held times 2^k, with k of each step from a bound on its norm n
+// (n <- n (|a| + |b| n^2 + |c| n^4) a step, at most 1 where k > 0), and the powers go into b, c and the result.
 //
 // A and Q = b A + c A A are symmetric: only tiles on and below the diagonal are computed.
 //
@@ -41,6 +43,29 @@ __device__ __forceinline__ void load2(const u32x4_t *p, int64_t frag, int lane, 
 
 // 1 / (|G| + eps); a matrix of zeros stays one, also with an eps of 0 or too small for its inverse.
 __device__ __forceinline__ double inverse_norm(double ss, double eps) { return ss == 0. ? 0. : 1. / (sqrt(ss) + eps); }
+// k of step 0: |X_0| 2^k in [0.5, 1); 0 for |X_0| of that size, zeros and what is not finite.
+__device__ __forceinline__ int first_power(double ss, double inv) {
+    const double n = sqrt(ss) * inv;
+    if (!(n > 0. && n < 0.5)) return 0;
+    int e;
+    frexp(n, &e);
+    return -e;
+}
+struct Growth {  // |a|, |b|, |c|
+    double a, b, c;
+};
+// k after s steps: a bound on |X| 2^k is at most 1, or k is 0.
+__device__ __forceinline__ int power_of(int k0, int s, Growth g) {
+    if (k0 == 0 && g.a >= 1.) return 0;  // as mostly
+    double n = ldexp(1. - 1e-9, -k0);    // (k0 again for s = 0)
+    for (int i = 0; i < s; ++i) {
+        n *= (g.a + n * n * (g.b + n * n * g.c)) * (1. + 1e-5);  // (roundings)
+        if (n >= 1.) return 0;
+    }
+    int e;
+    frexp(n, &e);
+    return n > 0. && n < 1. ? -e : 0;
+}
 
 // Four values as (hi, lo) halves.
 struct Quad {
@@ -93,7 +118,7 @@ __device__ __forceinline__ void get_block(const u32x4_t *src, int64_t row_block,
 // blocks (w >> 1) + 2 j in registers, in fp32, and block (w >> 1, w & 1) of A.
 template <class T, int NW>
 __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g, T *y, int32_t steps, float ca,
-                                                     float cb, float cc, double eps) {
+                                                     float cb, float cc, double eps, Growth gr) {
     constexpr int KL = 4 * NW;  // 16-column steps of X's rows
     __shared__ u32x4_t xs[2 * KL * 2 * 64], xt[2 * NW * 4 * 2 * 64], am[2 * 4 * 2 * 64], qm[2 * 4 * 2 * 64];
     double *red = reinterpret_cast<double *>(qm);  // qm is first written two barriers later
@@ -114,13 +139,15 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
     if (lane == 0) red[wave] = ss;
     __syncthreads();
-    const double inv = inverse_norm((red[0] + red[1]) + (red[2] + red[3]), eps);
+    ss = (red[0] + red[1]) + (red[2] + red[3]);
+    const double inv = inverse_norm(ss, eps);
+    const int k0 = first_power(ss, inv);
     constexpr float up = 1 << kScale, down = 1.f / (1 << kScale);
     // values in x are X 2^11, as the fragments hold them
 #pragma unroll
     for (int j = 0; j < NW; ++j)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[j][i] = (float)(x[j][i] * inv) * up;
+        for (int i = 0; i < 16; ++i) x[j][i] = (float)ldexp(x[j][i] * inv, k0) * up;
 
     auto store_x = [&]() {
         _Float16 *rows = reinterpret_cast<_Float16 *>(xs);
@@ -162,6 +189,8 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
     store_x();
     __syncthreads();
     for (int s = 0; s < steps; ++s) {
+        const int k = power_of(k0, s, gr), next = power_of(k0, s + 1, gr) - k;
+        const float kb = ldexpf(cb, -2 * k), kc = ldexpf(cc, -4 * k);
         float av[16], v[16];
         f32x16_t acc = product(xs, nb0 * KL, xs, mb * KL, std::integral_constant<int, KL>());
 #pragma unroll
@@ -170,14 +199,14 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
         __syncthreads();
         acc = product(am, nb0 * 4, am, mb * 4, std::integral_constant<int, 4>());
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = fmaf(cb, av[i], cc * (acc[i] * down));
+        for (int i = 0; i < 16; ++i) v[i] = fmaf(kb, av[i], kc * (acc[i] * down));
         put_block(qm, mb, 4, nb0 * 32, v, lane);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
             acc = product(qm, mb * 4, xt, (nb0 + 2 * j) * 4, std::integral_constant<int, 4>());
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[j][i] = fmaf(ca, x[j][i], acc[i] * down);
+            for (int i = 0; i < 16; ++i) x[j][i] = ldexpf(fmaf(ca, x[j][i], acc[i] * down), next);
         }
         if (s + 1 < steps) {
             __syncthreads();
@@ -186,18 +215,19 @@ __global__ __launch_bounds__(kThreads) void ns_small(Mat in, Mat out, const T *g
         }
     }
     T *dst = y + blockIdx.x * out.sb;
+    const int last = power_of(k0, steps, gr);
 #pragma unroll
     for (int j = 0; j < NW; ++j)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int64_t r = mb * 32 + 8 * (i >> 2) + 4 * h + (i & 3), c = (nb0 + 2 * j) * 32 + col;
-            if (r < out.S && c < out.L) dst[r * out.sr + c * out.sc] = (T)(x[j][i] * down);
+            if (r < out.S && c < out.L) dst[r * out.sr + c * out.sc] = (T)ldexpf(x[j][i] * down, -last);
         }
 }
 
 // ------------------------------------------------------------------ tiles over the whole chip
 
-constexpr int kSumBlocks = 256;  // partial sums of squares a matrix
+constexpr int kSumBlocks = 255;  // partial sums of squares a matrix; a matrix's 256th value is its first power
 
 template <class T>
 __global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double *part) {
@@ -229,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void ns_sumsq(Mat in, const T *g, double 
     for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.y * kSumBlocks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) part[blockIdx.y * (kSumBlocks + 1) + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 struct Work {  // fragment matrices of one matrix of the batch; the next one's follow at the strides
@@ -240,19 +270,22 @@ struct Work {  // fragment matrices of one matrix of the batch; the next one's f
 
 // 32 x 32 blocks of X_0 into both fragment matrices, zeros in the padding.
 template <class T>
-__global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const double *part, double eps, Work w) {
+__global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, double *part, double eps, Work w) {
     __shared__ float tile[4][32][33];
     __shared__ double red[4];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int64_t batch = blockIdx.y, nb = w.Lp / 32, blocks = nb * (w.Sp / 32);
-    static_assert(kSumBlocks == kThreads, "one partial sum a thread");
-    double ss = part[batch * kSumBlocks + t];  // joined in the same order by every workgroup
+    static_assert(kSumBlocks < kThreads, "one partial sum a thread");
+    double *sums = part + batch * (kSumBlocks + 1);
+    double ss = t < kSumBlocks ? sums[t] : 0.;  // joined in the same order by every workgroup
 #pragma unroll
     for (int o = 32; o; o >>= 1) ss += __shfl_xor(ss, o, 64);
     if (lane == 0) red[wave] = ss;
     __syncthreads();
     ss = (red[0] + red[1]) + (red[2] + red[3]);
     const double inv = inverse_norm(ss, eps);
+    const int k0 = first_power(ss, inv);
+    if (blockIdx.x == 0 && t == 0) sums[kSumBlocks] = (double)k0;
     const T *src = g + batch * in.sb;
     const int64_t blk = (int64_t)blockIdx.x * 4 + wave;
     const int64_t r0 = blk / nb * 32, c0 = blk % nb * 32;
@@ -263,7 +296,7 @@ __global__ __launch_bounds__(kThreads) void ns_pack(Mat in, const T *g, const do
             const int r = flip ? i & 31 : i >> 5, c = flip ? i >> 5 : i & 31;
             float v = 0.f;
             if (r0 + r < in.S && c0 + c < in.L)
-                v = (float)((double)(float)src[(r0 + r) * in.sr + (c0 + c) * in.sc] * inv) * (float)(1 << kScale);
+                v = (float)ldexp((double)(float)src[(r0 + r) * in.sr + (c0 + c) * in.sc] * inv, k0) * (float)(1 << kScale);
             tile[wave][r][c] = v;
         }
     }
@@ -303,14 +336,36 @@ struct Prod {
     const u32x4_t *add;       // what is added, with d0's layout
     int64_t badd;
     float f_add, f_mul;     // result = f_add add + f_mul product
+    const double *power;    // first powers, kSumBlocks + 1 apart
+    int32_t step;
+    Growth growth;
     int64_t splits, per;    // of the contraction, in 16-column steps (256-high tiles)
     float4 *part;
 };
 
+// The factors of a step's sums, with the powers of two that X and A are held times.
+struct Factors {
+    float add, mul;
+    int k;  // the result's power (kLast)
+};
+// (its first power is read at a kernel's start, so that no load stands between the products and their results)
+template <int MODE>
+__device__ __forceinline__ int power_at(const Prod &a, int64_t batch) {
+    return MODE == kGram ? 0 : __builtin_amdgcn_readfirstlane((int)a.power[batch * (kSumBlocks + 1)]);
+}
+template <int MODE>
+__device__ __forceinline__ Factors factors_of(const Prod &a, int k0) {
+    if constexpr (MODE == kGram) return {0.f, 1.f, 0};
+    const int k = power_of(k0, a.step, a.growth);
+    if constexpr (MODE == kPoly) return {ldexpf(a.f_add, -2 * k), ldexpf(a.f_mul, -4 * k), 0};
+    const int next = power_of(k0, a.step + 1, a.growth);
+    return {ldexpf(a.f_add, next - k), ldexpf(a.f_mul, next - k), next};
+}
+
 // One 32 x 32 block at (m0, n0): scaled, added to, written both ways.  `turn` is a wave's 32 x 33 floats.
 template <int MODE, class T>
 __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_t batch, int64_t m0, int64_t n0,
-                                     bool mirror, const f32x16_t &acc, float (*turn)[33], int lane) {
+                                     bool mirror, const Factors &f, const f32x16_t &acc, float (*turn)[33], int lane) {
     constexpr float down = 1.f / (1 << kScale);
     float v[16];
     if constexpr (MODE == kGram) {
@@ -319,7 +374,7 @@ __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_
     } else {
         get_block(a.add + batch * a.badd, n0 / 32, a.KS0, m0, v, lane);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = fmaf(a.f_add, v[i], a.f_mul * (acc[i] * down));
+        for (int i = 0; i < 16; ++i) v[i] = fmaf(f.add, v[i], f.mul * (acc[i] * down));
     }
     if constexpr (MODE == kLast) {
         T *dst = y + batch * out.sb;
@@ -327,7 +382,7 @@ __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int64_t r = m0 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-            if (r < out.S && c < out.L) dst[r * out.sr + c * out.sc] = (T)(v[i] * down);
+            if (r < out.S && c < out.L) dst[r * out.sr + c * out.sc] = (T)ldexpf(v[i] * down, -f.k);
         }
         return;
     }
@@ -342,11 +397,11 @@ __device__ __forceinline__ void emit(const Prod &a, const Mat &out, T *y, int64_
         float r[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) r[e] = turn[lane & 31][k * 16 + 8 * (lane >> 5) + e];
-        Frag2 f;
-        split8(r, f);
+        Frag2 fr;
+        split8(r, fr);
         u32x4_t *d = a.d1 + batch * a.b1 + ((m0 / 32 * a.KS1 + n0 / 16 + k) * 2) * 64 + lane;
-        d[0] = __builtin_bit_cast(u32x4_t, f.p[0]);
-        d[64] = __builtin_bit_cast(u32x4_t, f.p[1]);
+        d[0] = __builtin_bit_cast(u32x4_t, fr.p[0]);
+        d[64] = __builtin_bit_cast(u32x4_t, fr.p[1]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -386,6 +441,7 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
     const int64_t k0 = split * a.per, k1 = k0 + a.per < a.KS ? k0 + a.per : a.KS;
     int64_t tm, tn;
     if (!tile_of<MODE, 1>(a, tm, tn)) return;
+    const int k_first = power_at<MODE>(a, batch);
     const u32x4_t *p = a.p + batch * a.bp, *q = a.q + batch * a.bq;
     f32x16_t acc[BT][BT];
 #pragma unroll
@@ -434,7 +490,8 @@ __global__ __launch_bounds__(NW * 64) void ns_prod_split(Prod a, Mat out, T *y) 
         return;
     }
     const bool mirror = MODE == kUpdate || tm != tn;
-    emit<MODE, T>(a, out, y, batch, (tm * BT + wave / BT) * 32, (tn * BT + wave % BT) * 32, mirror, s,
+    emit<MODE, T>(a, out, y, batch, (tm * BT + wave / BT) * 32, (tn * BT + wave % BT) * 32, mirror,
+                  factors_of<MODE>(a, k_first), s,
                   reinterpret_cast<float (*)[33]>(&part[wave * (BT == 1 ? 2 : 1)][0][0][0]), lane);
 }
 
@@ -461,8 +518,9 @@ __global__ __launch_bounds__(BT * BT * 64) void ns_join_blocks(Prod a, Mat out, 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int64_t tm, tn;
     if (!tile_of<MODE, 1>(a, tm, tn)) return;
+    const int k_first = power_at<MODE>(a, blockIdx.y);
     emit<MODE, T>(a, out, y, blockIdx.y, (tm * BT + wave / BT) * 32, (tn * BT + wave % BT) * 32,
-                  MODE == kUpdate || tm != tn, join_block(a, blockIdx.y, wave, BT * BT, lane), turn[wave], lane);
+                  MODE == kUpdate || tm != tn, factors_of<MODE>(a, k_first), join_block(a, blockIdx.y, wave, BT * BT, lane), turn[wave], lane);
 }
 
 // Many tiles: 256 x 128 a workgroup, four waves of 128 x 64 (one a SIMD, half the register file in
@@ -480,6 +538,7 @@ __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y)
     const int64_t batch = blockIdx.y / a.splits, split = blockIdx.y % a.splits;
     int64_t tm, tn;
     if (!tile_of<MODE, 2>(a, tm, tn)) return;
+    const int k_first = power_at<MODE>(a, batch);
     const int64_t k0 = split * a.per, k1 = k0 + a.per < a.KS ? k0 + a.per : a.KS;
     // thread t stages 16 bytes of each row block: 256 threads are the block's 2 steps of 2 planes
     const u32x4_t *p = a.p + batch * a.bp + tm * 8 * a.KS * 128 + t;
@@ -577,9 +636,10 @@ __global__ __launch_bounds__(kThreads, 1) void ns_prod256(Prod a, Mat out, T *y)
     }
     const bool mirror = MODE == kUpdate || tn < 2 * tm;  // a square's own tiles hold both its triangles
     float(*turn)[33] = reinterpret_cast<float(*)[33]>(reinterpret_cast<float *>(&lds[0][0]) + wave * 32 * 33);
+    const Factors f = factors_of<MODE>(a, k_first);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        emit<MODE, T>(a, out, y, batch, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32, mirror,
+        emit<MODE, T>(a, out, y, batch, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32, mirror, f,
                       acc[i >> 1][i & 1], turn, lane);
 }
 
@@ -589,9 +649,10 @@ __global__ __launch_bounds__(kThreads) void ns_join(Prod a, Mat out, T *y) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wm = wave >> 1, wn = wave & 1;
     int64_t tm, tn;
     if (!tile_of<MODE, 2>(a, tm, tn)) return;
+    const int k_first = power_at<MODE>(a, blockIdx.y);
     const int i = blockIdx.z;  // one block of each wave's eight
     emit<MODE, T>(a, out, y, blockIdx.y, (tm * 8 + wm * 4 + (i >> 1)) * 32, (tn * 4 + wn * 2 + (i & 1)) * 32,
-                  MODE == kUpdate || tn < 2 * tm, join_block(a, blockIdx.y, wave * 8 + i, 32, lane), turn[wave], lane);
+                  MODE == kUpdate || tn < 2 * tm, factors_of<MODE>(a, k_first), join_block(a, blockIdx.y, wave * 8 + i, 32, lane), turn[wave], lane);
 }
 
 // ------------------------------------------------------------------ host side
@@ -636,20 +697,20 @@ inline Plan plan_of(int64_t batch, int64_t S, int64_t L) {
         const int64_t most = std::max(p.splits_gram, p.splits_poly);
         p.part = most > 1 ? batch * most * tri_tiles(p) * 256 * 128 / 4 : 0;
     }
-    p.bytes = batch * (3 * p.xsz + 2 * p.asz) * 16 + p.part * 16 + batch * kSumBlocks * 8;
+    p.bytes = batch * (3 * p.xsz + 2 * p.asz) * 16 + p.part * 16 + batch * (kSumBlocks + 1) * 8;
     return p;
 }
 
 template <class T>
 int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const void *g, void *y, int32_t steps, float ca,
-        float cb, float cc, double eps, void *ws, hipStream_t st) {
+        float cb, float cc, double eps, Growth growth, void *ws, hipStream_t st) {
     const T *src = static_cast<const T *>(g);
     T *dst = static_cast<T *>(y);
     if (p.small) {
         const dim3 gr((unsigned)batch), b(kThreads);
-        if (in.L <= 64) hipLaunchKernelGGL((ns_small<T, 1>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps);
-        else if (in.L <= 128) hipLaunchKernelGGL((ns_small<T, 2>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps);
-        else hipLaunchKernelGGL((ns_small<T, 4>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps);
+        if (in.L <= 64) hipLaunchKernelGGL((ns_small<T, 1>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps, growth);
+        else if (in.L <= 128) hipLaunchKernelGGL((ns_small<T, 2>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps, growth);
+        else hipLaunchKernelGGL((ns_small<T, 4>), gr, b, 0, st, in, out, src, dst, steps, ca, cb, cc, eps, growth);
         return launch_status(fn);
     }
     Work w{};
@@ -670,6 +731,7 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
     const int64_t ts = p.Sp / p.tile, tl = p.Lp / (p.tile == 256 ? 128 : p.tile);
     const int64_t tri = tri_tiles(p), all = ts * tl;
     const int64_t ks = p.Sp / 16, kl = p.Lp / 16;
+    const double *power = part + kSumBlocks;
     auto go = [&](auto mode, Prod a, int64_t splits) {
         constexpr int M = decltype(mode)::value;
         const unsigned n = (unsigned)((a.tiles + 7) / 8 * 8);
@@ -691,12 +753,12 @@ int run(const char *fn, const Plan &p, int64_t batch, Mat in, Mat out, const voi
     for (int32_t s = 0; s < steps; ++s) {
         u32x4_t *cur = w.xt[s & 1], *nxt = w.xt[(s + 1) & 1];
         go(std::integral_constant<int, kGram>(),
-           Prod{w.x, w.x, w.bx, w.bx, kl, tri, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f, 1, 0, nullptr},
+           Prod{w.x, w.x, w.bx, w.bx, kl, tri, 0, w.a, w.a, ks, ks, w.ba, w.ba, nullptr, 0, 0.f, 1.f, power, s, growth, 1, 0, nullptr},
            p.splits_gram);
         go(std::integral_constant<int, kPoly>(),
-           Prod{w.a, w.a, w.ba, w.ba, ks, tri, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc, 1, 0, nullptr},
+           Prod{w.a, w.a, w.ba, w.ba, ks, tri, 0, w.q, w.q, ks, ks, w.ba, w.ba, w.a, w.ba, cb, cc, power, s, growth, 1, 0, nullptr},
            p.splits_poly);
-        const Prod u{w.q, cur, w.ba, w.bx, ks, all, ts, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f, 1, 0, nullptr};
+        const Prod u{w.q, cur, w.ba, w.bx, ks, all, ts, nxt, w.x, ks, kl, w.bx, w.bx, cur, w.bx, ca, 1.f, power, s, growth, 1, 0, nullptr};
         if (s + 1 < steps) go(std::integral_constant<int, kUpdate>(), u, 1);
         else go(std::integral_constant<int, kLast>(), u, 1);
     }
@@ -839,8 +901,9 @@ extern "C" int igr_newton_schulz(int32_t dtype, int64_t batch, int64_t rows, int
         const Mat to{S, L, flip ? 1 : cols, flip ? cols : 1, rows * cols};
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
         const float fa = (float)a, fb = (float)b, fc = (float)c;
-        if (dtype == kF32) return run<float>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, workspace, st);
-        if (dtype == kBF16) return run<__bf16>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, workspace, st);
-        return run<_Float16>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, workspace, st);
+        const Growth growth{std::fabs(a), std::fabs(b), std::fabs(c)};
+        if (dtype == kF32) return run<float>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, growth, workspace, st);
+        if (dtype == kBF16) return run<__bf16>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, growth, workspace, st);
+        return run<_Float16>(fn, p, batch, in, to, g, out, steps, fa, fb, fc, eps, growth, workspace, st);
     });
 }
