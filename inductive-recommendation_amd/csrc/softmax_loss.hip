@@ -26,10 +26,10 @@
 // in registers and batch blocks streamed; no atomics on memory, the same bits on every run.
 //
 // Bound by the matrix cores and, beside them, the softmax's own arithmetic (an exponential, a
-// subtraction and two conversions a weight).  B = 2048, d = 64, fp32: one million items take 1.54 ms
-// forward and 1.39 ms backward, 1.0 and 1.1 PFLOP/s of fp16 products.  On operands that are not constant
+// subtraction and two conversions a weight).  B = 2048, d = 64, fp32: one million items take 1.44 to 1.54 ms
+// forward and 1.32 to 1.39 backward (from card to card), 1.0 to 1.2 PFLOP/s of fp16 products.  On operands that are not constant
 // MFMAs alone sustain 1.56 here (2.3 on constants: the clock falls with what they switch), a large
-// library product 1.55.  40,981 items take 81 and 90 us; at d = 256 (one wave a SIMD) 0.35 and 0.31 ms
+// library product 1.55.  40,981 items take 82 and 91 us; at d = 256 (one wave a SIMD) 0.35 and 0.31 ms
 // with the small kernels.
 //
 // fp32 in fewer bits than fp32's: operands are pairs of halves (2^-23, the rows' own powers of two), and an
