@@ -27,14 +27,14 @@
 //
 // Bound by the matrix cores and, beside them, the softmax's own arithmetic (an exponential, a
 // subtraction and two conversions a weight).  B = 2048, d = 64, fp32: one million items take 1.44 to 1.54 ms
-// forward and 1.32 to 1.39 backward (from card to card), 1.0 to 1.2 PFLOP/s of fp16 products.  On operands that are not constant
-// MFMAs alone sustain 1.56 here (2.3 on constants: the clock falls with what they switch), a large
-// library product 1.55.  40,981 items take 82 and 91 us; at d = 256 (one wave a SIMD) 0.35 and 0.31 ms
-// with the small kernels.
+// forward and 1.32 to 1.39 backward (from card to card), 1.0 to 1.2 PFLOP/s of fp16 products.  On operands
+// that are not constant MFMAs alone sustain 1.56 here (2.3 on constants: the clock falls with what they
+// switch), a large library product 1.55.  40,981 items take 82 and 93 us; at d = 256 (one wave a SIMD) 0.35
+// and 0.31 ms with the small kernels.
 //
-// fp32 in fewer bits than fp32's: operands are pairs of halves (2^-23, the rows' own powers of two), and an
-// exponent's argument, which log-sum, coefficient and power of two go into together, is one
-// fp32 of up to 40, so that a row's weights in dw share an error of up to 2^-20.
+// fp32 in fewer bits than fp32's: operands are pairs of halves (2^-23, the rows' own powers of two).  Of half
+// types the argument of an exponent in the backward, which log-sum, coefficient and power of two go into
+// together, is one fp32 of up to 40, so that a row's weights in dw share an error of up to 2^-20.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -58,11 +58,11 @@ __host__ __device__ constexpr int block_halves(int dp) { return 2 * P::NS * kRB 
 inline int64_t block_bytes(int32_t dtype, int dp) { return (dtype == kF32 ? 2 : 1) * 2ll * kRB * dp * 2; }
 inline int64_t align256(int64_t n) { return (n + 255) & ~255ll; }
 
-// A packed table: its blocks, then (of the batch) what fp32 leaves of the rows' log-sums, and fp32's exponents: a row's entries are held times 2^(14 - its own).  A block
-// whose rows are within 2^kNarrow of each other has one exponent for all of them (its largest row's), and
-// the kernels their short path; the digits of a row 2^8 below it still reach 2^-31 of its largest entry.  In
-// the others each row has its own, however large its neighbours are (an item masked by
-// an entry of -1e9 or the type's lowest value).
+// A packed table: its blocks, then fp32's exponents, then (of the batch, for the backward) what fp32 left of the rows'
+// log-sums.  A row's entries are held times 2^(14 - its exponent).  A block whose rows are within 2^kNarrow of
+// each other has one exponent for all of them (its largest row's), and the kernels their short path; the digits
+// of a row 2^8 below it still reach 2^-31 of its largest entry.  In the others each row has its own, however
+// large its neighbours are (an item masked by an entry of -1e9 or the type's lowest value).
 struct Packed {
     const u32x4_t *blocks;
     const int32_t *exps;      // per block: its largest row's, plus kWide where rows have their own
@@ -76,7 +76,8 @@ inline Packed packed_view(const void *p, int64_t rows, int32_t dtype, int dp) {
                   reinterpret_cast<const int8_t *>(c + blocks_of(rows) * sizeof(int32_t)),
                   reinterpret_cast<const int16_t *>(c + blocks_of(rows) * (sizeof(int32_t) + kRB))};
 }
-// lse2 is off by half its fp32 step at most, and by no more than the log of a sum, below 32: 2^-15 of that.
+// lse2, a maximum and the log of a sum (below 32) in one fp32, is off by half its step or that log at most:
+// 2^-15 of it.
 __device__ __forceinline__ float rest_unit(float lse2) {
     const int step = (int)((__builtin_bit_cast(uint32_t, lse2) >> 23) & 255u) - 127 - 24;  // of half a step
     return ldexpf(1.f, min(step, 5) - 15);
@@ -322,6 +323,7 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 || !WITH_O ? 2 : 1)) v
         // this wave's batch blocks
         Frags<P> xf[NB][KS];
         // top: the largest log2 of a weight (relative to m) times its row's power of two so far; far: some |m| is
+        // beyond kFar
         float c_x[NB], m[NB], top[NB], z[NB], tl[NB];
         int tgt[NB];
         bool live[NB], far[NB];
@@ -630,14 +632,16 @@ __global__ __launch_bounds__(kReduceThreads) void softmax_reduce(int64_t B, cons
     }
 }
 
-// What the streamed batch blocks of the backward carry besides their fragments, per row: the
-// exponent offset that makes exp2(acc c - off) = |c_b| p 2^(14 + e - C), the same power of c_b r_b for
-// the target's own term (with c_b's sign, zero or not), the target.
+// What the streamed batch blocks of the backward carry besides their fragments, per row: lse2 and what stands
+// beside it to make exp2(acc c - lse + beside) = |c_b| p 2^(14 + e - C), the same power of c_b r_b for the
+// target's own term (with c_b's sign, zero or not), the target.  off is the two in one fp32, off by half the
+// step of up to 40, 2^-20, for all of a row's weights: the half types take it, whose results round further
+// (1500 x 50,021 x 200 in bf16: 140 us backward, 166 from the two), fp32 does not (2048 x a million x 64: dw
+// off by 9.7e-7 of its norm, 7.7e-7 to 8.5e-7 from the two; 1.35 and 1.36 ms).
 struct RowInfo {
-    float *off, *hot;
+    float *lse, *beside, *hot, *off;
     int32_t *tgt;
     int32_t *flags; // per block: kMinus, some c_b < 0; kFarRows, some |lse2| > kFar
-    float2 *apart;  // lse2 as it is, and what off has beside it
     int32_t *cmax;  // C: the largest e + floor(log2 |c_b|)
     int32_t *part;  // kScanGroups partial maxima
 };
@@ -729,28 +733,27 @@ __global__ __launch_bounds__(kThreads) void softmax_coef(CoefArgs a) {
     const int C = cm;
     const int64_t b = id * kThreads + t;
     if (b >= blocks_of(a.B) * kRB) return;
-    float off = INFINITY, hot = 0.f;
+    float lse = 0.f, beside = -INFINITY, hot = 0.f;
     int tgt = -1;
     bool minus = false, far = false;
-    float2 apart = make_float2(0.f, -INFINITY);
     if (b < a.B) {
         const int64_t tg = a.target[b];
         const float c = row_coef(a, b, tg);
         const int e = SCALED ? a.x.row_exps[b] : 0;
         if (c != 0.f) {
-            const float lse = a.lse2[b], rest = log2f(fabsf(c)) + (float)(14 + e - C);
-            off = lse - rest;
+            lse = a.lse2[b];
+            beside = log2f(fabsf(c)) + (float)(14 + e - C) - (float)a.x.lse_rest[b] * rest_unit(lse);
             far = fabsf(lse) > kFar;
-            apart = make_float2(lse, rest - (float)a.x.lse_rest[b] * rest_unit(lse));
             hot = ldexpf(c * a.rest[b], 14 + e - C);
             minus = c < 0.f;
             tgt = tg >= 0 && tg < a.V ? (int)tg : -1;
         }
     }
-    a.info.off[b] = off;
+    a.info.off[b] = lse - beside;
     a.info.hot[b] = hot;
     a.info.tgt[b] = tgt;
-    a.info.apart[b] = apart;
+    a.info.lse[b] = lse;
+    a.info.beside[b] = beside;
     const uint64_t neg = __ballot(minus), wide = __ballot(far);
     if ((lane & 31) == 0)
         a.info.flags[b / kRB] = ((uint32_t)(neg >> lane) ? kMinus : 0) | ((uint32_t)(wide >> lane) ? kFarRows : 0);
@@ -789,7 +792,9 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
     constexpr int KS = DP / 16, DB = DP / 32;
     constexpr int BLK = block_halves<P>(DP) / 8;
     __shared__ u32x4_t lds0[BLK], lds1[BLK];
-    __shared__ float info0[3][kRB], info1[3][kRB];  // off, hot, target of the streamed block
+    constexpr int kInfo = P::NS == 1 ? 5 : 4;
+    // lse, beside, hot, target (, off) of the streamed block
+    __shared__ __align__(16) float info0[kInfo][kRB], info1[kInfo][kRB];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 31, h = lane >> 5;
     const int64_t nvb = blocks_of(a.V), nxb = blocks_of(a.B);
     const int64_t split = blockIdx.y;
@@ -818,9 +823,11 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
     // As in the forward: x and info in use, the next ones filled meanwhile, two arrays by name.
     auto fetch_info = [&](int64_t k) {
         float v = 0.f;
-        if (t < kRB) v = a.info.off[k * kRB + t];
-        else if (t < 2 * kRB) v = a.info.hot[k * kRB + t - kRB];
-        else if (t < 3 * kRB) v = __builtin_bit_cast(float, a.info.tgt[k * kRB + t - 2 * kRB]);
+        if (t < kRB) v = a.info.lse[k * kRB + t];
+        else if (t < 2 * kRB) v = a.info.beside[k * kRB + t - kRB];
+        else if (t < 3 * kRB) v = a.info.hot[k * kRB + t - 2 * kRB];
+        else if (t < 4 * kRB) v = __builtin_bit_cast(float, a.info.tgt[k * kRB + t - 3 * kRB]);
+        else if (kInfo == 5 && t < 5 * kRB) v = a.info.off[k * kRB + t - 4 * kRB];
         return v;
     };
     int e_next = P::kScaled ? a.x.exps[k0] : 0, flags_next = a.info.flags[k0];
@@ -850,38 +857,38 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
 #pragma unroll
                 for (int n = 0; n < NB; ++n) acc[n][i] = ldexpf(acc[n][i], e - e_x);
             });
-        const int tcol = __builtin_bit_cast(int, info[2][col]);
+        const int tcol = __builtin_bit_cast(int, info[3][col]);
         Frags<P> pf[NB][2];
         Frags<P> rest[NB][P::NS == 1 ? 2 : 1];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             const float c = c_w[n] * c_x;
             float p[16];
-            if (flags & kFarRows) {  // equal logits as in the forward: one less the other is 0
-                const volatile float2 *apart = a.info.apart + k * kRB + 4 * h;
+            auto weights = [&](auto exponent, int first) {  // exponent(logit / c, the row's lse or off, its beside)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float lse = apart[8 * (i >> 2) + (i & 3)].x, rest = apart[8 * (i >> 2) + (i & 3)].y;
-                    p[i] = __builtin_amdgcn_exp2f((rounded_product(acc[n][i], c) - lse) + rest);
+                for (int g = 0; g < 4; ++g) {
+                    const float4 l = *reinterpret_cast<const float4 *>(&info[first][8 * g + 4 * h]);
+                    const float4 b = *reinterpret_cast<const float4 *>(&info[1][8 * g + 4 * h]);
+                    p[4 * g] = __builtin_amdgcn_exp2f(exponent(acc[n][4 * g], l.x, b.x));
+                    p[4 * g + 1] = __builtin_amdgcn_exp2f(exponent(acc[n][4 * g + 1], l.y, b.y));
+                    p[4 * g + 2] = __builtin_amdgcn_exp2f(exponent(acc[n][4 * g + 2], l.z, b.z));
+                    p[4 * g + 3] = __builtin_amdgcn_exp2f(exponent(acc[n][4 * g + 3], l.w, b.w));
                 }
-            } else
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4 off = *reinterpret_cast<const float4 *>(&info[0][8 * g + 4 * h]);
-                p[4 * g] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g], c, -off.x));
-                p[4 * g + 1] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g + 1], c, -off.y));
-                p[4 * g + 2] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g + 2], c, -off.z));
-                p[4 * g + 3] = __builtin_amdgcn_exp2f(fmaf(acc[n][4 * g + 3], c, -off.w));
-            }
+            };
+            // (far: equal logits as in the forward, one less the other is 0)
+            if (flags & kFarRows)
+                weights([&](float s, float lse, float b) { return rounded_product(s, c) - lse + b; }, 0);
+            else if constexpr (kInfo == 5) weights([&](float s, float off, float) { return fmaf(s, c, -off); }, 4);
+            else weights([&](float s, float lse, float b) { return fmaf(s, c, -lse) + b; }, 0);
             if (neg) {  // a negative c_b: only where the caller's gradients are
 #pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = copysignf(p[i], info[1][8 * (i >> 2) + 4 * h + (i & 3)]);
+                for (int i = 0; i < 16; ++i) p[i] = copysignf(p[i], info[2][8 * (i >> 2) + 4 * h + (i & 3)]);
             }
             if (__any((unsigned)(tcol - v0[n]) < 32u)) {  // some row's target is one of these items
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int r = 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (__builtin_bit_cast(int, info[2][r]) == v0[n] + col) p[i] = -info[1][r];
+                    if (__builtin_bit_cast(int, info[3][r]) == v0[n] + col) p[i] = -info[2][r];
                 }
             }
             split_weights<P>(p, pf[n], rest[n]);
@@ -894,12 +901,12 @@ __global__ __launch_bounds__(kThreads, (DP * P::NS <= 256 ? 2 : 1)) void softmax
             mfma_row<P, NB>(xf, [&](int n) -> const Frags<P> & { return pf[n][f & 1]; }, of);
             if constexpr (P::NS == 1) mfma_row<P, NB>(xf, [&](int n) -> const Frags<P> & { return rest[n][f & 1]; }, of);
         }
-        if (k + 1 < k1 && t < 3 * kRB) info_next[t / kRB][t % kRB] = si;
+        if (k + 1 < k1 && t < kInfo * kRB) info_next[t / kRB][t % kRB] = si;
         copies_done();
         __syncthreads();
     };
     copy_to_lds<BLK>(a.x.blocks + k0 * BLK, lds0, t);
-    if (t < 3 * kRB) info0[t / kRB][t % kRB] = fetch_info(k0);
+    if (t < kInfo * kRB) info0[t / kRB][t % kRB] = fetch_info(k0);
     copies_done();
     __syncthreads();
     for (int64_t k = k0; k < k1; k += 2) {
@@ -1023,11 +1030,12 @@ BwdArgs bwd_args(Carve &c, int64_t b, int64_t v, int dp) {
     BwdArgs a{};
     a.B = b, a.V = v, a.splits = p.splits, a.per = p.per;
     const int64_t rows = blocks_of(b) * kRB;
-    a.info.off = c.take<float>(rows);
     a.info.hot = c.take<float>(rows);
     a.info.tgt = c.take<int32_t>(rows);
     a.info.flags = c.take<int32_t>(rows / kRB);
-    a.info.apart = c.take<float2>(rows);
+    a.info.lse = c.take<float>(rows);
+    a.info.off = c.take<float>(rows);
+    a.info.beside = c.take<float>(rows);
     a.info.cmax = c.take<int32_t>(1);
     a.info.part = c.take<int32_t>(kScanGroups);
     a.part = p.splits > 1 ? c.take<float>(p.splits * v * dp) : nullptr;
